@@ -35,6 +35,11 @@ extern "C" {
 #define LGD_EINVAL (-1)   /* bad argument (null pointer, L > LGD_MAX_LEVELS, C % 4 != 0, ...) */
 #define LGD_ELAUNCH (-2)  /* hipLaunchKernel reported an error */
 
+/* element types of the entry points that take more than fp32 */
+#define LGD_F32 0
+#define LGD_BF16 1
+#define LGD_F16 2
+
 /* ABI version, bumped on any signature change. */
 int lgd_abi_version(void);
 /* Name of the GPU arch the library was compiled for ("gfx950"). */
@@ -605,6 +610,55 @@ typedef struct lgd_sgd_tensor {
 int lgd_sgd_chunk_elems(void);
 int lgd_sgd_clip_step(const lgd_sgd_tensor* table, const int32_t* blk_off, int n_tensors, int n_blocks, float clip_value,
                       void* stream);
+
+/* ------------------------------------------------------------------ gradient norm over many tensors, and clipping by it
+ * norm_type: LGD_NORM_2 sqrt(sum g^2), LGD_NORM_1 sum |g|, LGD_NORM_INF max |g| (a NaN anywhere gives NaN), over every element of
+ * every tensor; sums in fp64, in a fixed order (no atomics: the same tensors give the same bits).
+ * lgd_grad_norm : *norm_out (device, 1 fp32) = the norm.
+ * lgd_grad_clip : the same, and every element g <- g * min(1, max_norm / (norm + 1e-6)), rounded once to the tensor's type.  Where the
+ *                 factor is 1 nothing is written.  The tensors must not overlap.  max_norm >= 0.
+ * tensors_host: HOST array of n records, consumed before the call returns (it travels in kernel arguments: no copy, safe to capture);
+ * p aligned to the element.  ws: lgd_grad_norm_ws_bytes(n) bytes, 8-byte aligned, contents irrelevant.
+ */
+#define LGD_NORM_2 0
+#define LGD_NORM_1 1
+#define LGD_NORM_INF 2
+typedef struct lgd_grad_tensor {
+    void* p;           /* elements, contiguous */
+    int64_t n;         /* their number */
+    int32_t dtype;     /* LGD_F32 / LGD_BF16 / LGD_F16 */
+    int32_t reserved;
+} lgd_grad_tensor;
+size_t lgd_grad_norm_ws_bytes(int n_tensors);
+int lgd_grad_norm(const lgd_grad_tensor* tensors_host, int n_tensors, int norm_type, void* ws, float* norm_out, void* stream);
+int lgd_grad_clip(const lgd_grad_tensor* tensors_host, int n_tensors, int norm_type, float max_norm, void* ws, float* norm_out,
+                  void* stream);
+/* lgd_sgd_clip_step with clipping by norm instead of by value: tensors [group_off_host[k], group_off_host[k + 1]) of the table form group k
+ * (the parameters of one optimizer; at most LGD_MAX_SGD_GROUPS), each clipped by its own norm -- g <- g * min(1, max_norm / (norm_k + 1e-6)),
+ * written back where the factor is not 1 -- before the update.  `reserved` of every record holds its group.  norms_out: n_groups fp32 (device);
+ * ws: lgd_sgd_norm_ws_bytes(n_groups) bytes, 8-byte aligned. */
+#define LGD_MAX_SGD_GROUPS 16
+size_t lgd_sgd_norm_ws_bytes(int n_groups);
+int lgd_sgd_norm_step(const lgd_sgd_tensor* table, const int32_t* blk_off, int n_tensors, int n_blocks, const int32_t* group_off_host,
+                      const int32_t* group_blk_host /* blk_off at the group borders, n_groups + 1 entries */, int n_groups, int norm_type,
+                      float max_norm, void* ws, float* norms_out, void* stream);
+
+/* ------------------------------------------------------------------ GroupNorm + activation, channels last
+ * GroupNorm(G, per-channel affine) then act over L maps stored (B, H_l, W_l, C), one module for all of them; dtype LGD_F32 / LGD_BF16 /
+ * LGD_F16 for x, y, dy, dx; gamma / beta (C entries, either may be NULL = 1 / 0) and their gradients in param_dtype.
+ * act: LGD_ACT_NONE, LGD_ACT_RELU, LGD_ACT_SILU.  All pointers aligned to the element (16 bytes is fastest); H_l * W_l * C below 2^31.
+ *   stats: fp64 [L*B*G][2] (mean, 1/sqrt(var + eps)), written by fwd, read by bwd;  ws: lgd_gn_act_ws_bytes(..., backward) bytes, 8-byte aligned
+ * backward: dx_host NULL: no input gradients; dgamma / dbeta NULL: not wanted.  Sums run in a fixed order (no atomics).
+ */
+#define LGD_ACT_NONE 0
+#define LGD_ACT_RELU 1
+#define LGD_ACT_SILU 2
+size_t lgd_gn_act_ws_bytes(const int32_t* level_hw_host, int L, int B, int C, int G, int dtype, int backward);
+int lgd_gn_act_fwd(const void* const* x_host, const int32_t* level_hw_host, int L, int B, int C, int G, int dtype, const void* gamma,
+                   const void* beta, int param_dtype, double eps, int act, void* ws, double* stats, void* const* y_host, void* stream);
+int lgd_gn_act_bwd(const void* const* x_host, const void* const* dy_host, const int32_t* level_hw_host, int L, int B, int C, int G,
+                   int dtype, const void* gamma, const void* beta, int param_dtype, int act, const double* stats, void* ws,
+                   void* const* dx_host, void* dgamma, void* dbeta, void* stream);
 
 /* ------------------------------------------------------------------ per-kernel timing (bench.py)
  * When enabled every kernel launch of this library is bracketed by a HIP event pair recorded on

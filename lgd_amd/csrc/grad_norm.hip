@@ -1,0 +1,181 @@
+// Norm over every element of many tensors (fp32 / bf16 / fp16, mixed, any sizes and alignments), and clipping by it in place.
+// Memory bound: the norm reads N bytes, clipping reads them twice and writes them (the factor depends on all of them).
+// The tensors are cut into chunks of 32 KB, numbered through; a fixed grid of workgroups takes equal contiguous runs of chunks and leaves one partial
+// word each, which the next kernel's workgroups all reduce for themselves (8 KB out of the L2): two launches, no atomics, the same bits every time.
+// The list travels in the kernel arguments (no host-to-device copy: nothing to wait for, nothing a captured graph could find overwritten); beyond
+// kNormInline tensors small kernels store it into the workspace first.
+#include "grad_norm.h"
+
+namespace lgd {
+
+constexpr int kNormChunk = 32768;    // bytes
+constexpr int kNormGrid = 1024;      // workgroups at most: 4 per CU, 16 waves of 8 x 16 bytes in flight
+constexpr int kNormInline = 160;     // records in the kernel arguments (24 bytes each, under 4 KB)
+
+struct NormEntry {
+    void* p;
+    long long n;
+    int blk0;        // number of its first chunk
+    int dtype;
+};
+struct NormTable {
+    NormEntry e[kNormInline];
+    const NormEntry* more;   // the whole table, when it does not fit
+    int n, nblk;
+};
+
+__device__ __forceinline__ NormEntry norm_entry(const NormTable& t, int i) { return t.more ? t.more[i] : t.e[i]; }
+__device__ __forceinline__ int norm_blk0(const NormTable& t, int i) { return t.more ? t.more[i].blk0 : t.e[i].blk0; }
+
+// the chunks of workgroup `w` of `grid`: f(entry, first element, number of elements)
+template <typename F>
+__device__ __forceinline__ void norm_walk(const NormTable& t, int w, int grid, F f) {
+    const int c0 = (int)((long long)t.nblk * w / grid), c1 = (int)((long long)t.nblk * (w + 1) / grid);
+    int lo = 0, hi = t.n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (norm_blk0(t, mid) <= c0) lo = mid; else hi = mid;
+    }
+    for (int c = c0; c < c1;) {
+        const NormEntry e = norm_entry(t, lo);
+        const int per = e.dtype == LGD_F32 ? kNormChunk / 4 : kNormChunk / 2;
+        const int last = min(c1, e.blk0 + (int)((e.n + per - 1) / per));
+        for (; c < last; ++c) {
+            const long long first = (long long)(c - e.blk0) * per;
+            f(e, first, (int)(e.n - first < per ? e.n - first : per));
+        }
+        ++lo;
+    }
+}
+
+__global__ __launch_bounds__(256) void norm_table_kernel(NormTable t, NormEntry* dst) {
+    for (int i = threadIdx.x; i < t.n; i += 256) dst[i] = t.e[i];
+}
+
+template <int NT>
+__global__ __launch_bounds__(256) void norm_partial_kernel(NormTable t, double* part) {
+    __shared__ double sh[4];
+    NormAcc<NT> acc;
+    norm_walk(t, blockIdx.x, gridDim.x, [&](const NormEntry& e, long long first, int count) {
+        if (e.dtype == LGD_F32) norm_chunk<NT, float, 8>(static_cast<const float*>(e.p) + first, count, acc);
+        else if (e.dtype == LGD_BF16) norm_chunk<NT, __bf16, 8>(static_cast<const __bf16*>(e.p) + first, count, acc);
+        else norm_chunk<NT, _Float16, 8>(static_cast<const _Float16*>(e.p) + first, count, acc);
+    });
+    acc = norm_block<NT>(acc, sh);
+    if (threadIdx.x == 0) part[blockIdx.x] = acc.word();
+}
+
+template <int NT>
+__global__ __launch_bounds__(256) void norm_final_kernel(const double* part, int np, float* out) {
+    __shared__ double sh[4];
+    const float v = norm_total<NT>(part, np, sh);
+    if (threadIdx.x == 0) *out = v;
+}
+
+template <typename T, int U>
+__device__ __forceinline__ void norm_scale_chunk(T* p, int count, float c) {
+    constexpr int V = Vec16<T>::V;
+    const int t = threadIdx.x, head = norm_head(p, count), nv = (count - head) / V, tail = head + nv * V;
+    if (t < head) p[t] = (T)((float)p[t] * c);
+    if (t < count - tail) p[tail + t] = (T)((float)p[tail + t] * c);
+    lgd_u32x4* q = reinterpret_cast<lgd_u32x4*>(p + head);
+    for (int i0 = t; i0 < nv; i0 += 256 * U) {
+        lgd_u32x4 v[U];
+        #pragma unroll
+        for (int u = 0; u < U; ++u) if (i0 + u * 256 < nv) v[u] = q[i0 + u * 256];
+        #pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (i0 + u * 256 >= nv) continue;
+            float f[V];
+            Vec16<T>::unpack(v[u], f);
+            #pragma unroll
+            for (int i = 0; i < V; ++i) f[i] *= c;
+            q[i0 + u * 256] = Vec16<T>::pack(f);
+        }
+    }
+}
+
+template <int NT>
+__global__ __launch_bounds__(256) void norm_scale_kernel(NormTable t, const double* part, int np, float max_norm, float* out) {
+    __shared__ double sh[4];
+    const float norm = norm_total<NT>(part, np, sh), c = norm_coef(norm, max_norm);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *out = norm;
+    if (c == 1.f) return;
+    norm_walk(t, blockIdx.x, gridDim.x, [&](const NormEntry& e, long long first, int count) {
+        if (e.dtype == LGD_F32) norm_scale_chunk<float, 8>(static_cast<float*>(e.p) + first, count, c);
+        else if (e.dtype == LGD_BF16) norm_scale_chunk<__bf16, 8>(static_cast<__bf16*>(e.p) + first, count, c);
+        else norm_scale_chunk<_Float16, 8>(static_cast<_Float16*>(e.p) + first, count, c);
+    });
+}
+
+static size_t norm_ws_part() { return (size_t)kNormGrid * sizeof(double); }
+
+// host list -> table (empty tensors dropped); LGD_EINVAL where a record is unusable.  *grid = workgroups
+static int norm_table(NormTable& t, const lgd_grad_tensor* host, int n, void* ws, hipStream_t s, int* grid) {
+    NormEntry* dev = reinterpret_cast<NormEntry*>(static_cast<char*>(ws) + norm_ws_part());
+    int live = 0;
+    for (int i = 0; i < n; ++i) {
+        const lgd_grad_tensor& h = host[i];
+        if (h.n < 0 || h.dtype < 0 || h.dtype > 2 || (h.n > 0 && (!h.p || reinterpret_cast<uintptr_t>(h.p) % (h.dtype == LGD_F32 ? 4 : 2)))) return LGD_EINVAL;
+        live += h.n > 0;
+    }
+    t.n = 0; t.more = nullptr;
+    long long blk = 0;
+    int done = 0;
+    for (int i = 0; i < n; ++i) {
+        const lgd_grad_tensor& h = host[i];
+        if (h.n == 0) continue;
+        const int per = h.dtype == LGD_F32 ? kNormChunk / 4 : kNormChunk / 2;
+        NormEntry& e = t.e[t.n++];
+        e.p = h.p; e.n = h.n; e.blk0 = (int)blk; e.dtype = h.dtype;
+        blk += (h.n + per - 1) / per;
+        if (blk > 0x3fffffffLL) return LGD_EINVAL;
+        if (live > kNormInline && (t.n == kNormInline || done + t.n == live)) {
+            LGD_LAUNCH("grad_norm_table_kernel", norm_table_kernel, dim3(1), dim3(256), 0, s, t, dev + done);
+            done += t.n; t.n = 0;
+        }
+    }
+    if (live > kNormInline) t.more = dev;
+    t.n = live; t.nblk = (int)blk;
+    *grid = blk < kNormGrid ? (blk < 1 ? 1 : (int)blk) : kNormGrid;
+    return LGD_OK;
+}
+
+template <int NT>
+static int norm_run(const NormTable& t, int grid, bool clip, float max_norm, void* ws, float* out, hipStream_t s) {
+    double* part = static_cast<double*>(ws);
+    LGD_LAUNCH("grad_norm_kernel", norm_partial_kernel<NT>, dim3((unsigned)grid), dim3(256), 0, s, t, part);
+    if (clip) LGD_LAUNCH("grad_clip_kernel", norm_scale_kernel<NT>, dim3((unsigned)grid), dim3(256), 0, s, t, part, grid, max_norm, out);
+    else LGD_LAUNCH("grad_norm_final_kernel", norm_final_kernel<NT>, dim3(1), dim3(256), 0, s, part, grid, out);
+    return check_launch();
+}
+
+static int norm_call(const lgd_grad_tensor* host, int n, int norm_type, bool clip, float max_norm, void* ws, float* out, void* stream) {
+    if (n < 0 || (n > 0 && !host) || norm_type < 0 || norm_type > 2 || !ws || !out || !(max_norm >= 0.f)) return LGD_EINVAL;
+    hipStream_t s = (hipStream_t)stream;
+    NormTable t;
+    int grid = 0;
+    const int rc = norm_table(t, host, n, ws, s, &grid);
+    if (rc != LGD_OK) return rc;
+    if (norm_type == LGD_NORM_2) return norm_run<LGD_NORM_2>(t, grid, clip, max_norm, ws, out, s);
+    if (norm_type == LGD_NORM_1) return norm_run<LGD_NORM_1>(t, grid, clip, max_norm, ws, out, s);
+    return norm_run<LGD_NORM_INF>(t, grid, clip, max_norm, ws, out, s);
+}
+
+}  // namespace lgd
+
+extern "C" {
+
+size_t lgd_grad_norm_ws_bytes(int n_tensors) {
+    return lgd::norm_ws_part() + (n_tensors > lgd::kNormInline ? (size_t)n_tensors * sizeof(lgd::NormEntry) : 0);
+}
+
+int lgd_grad_norm(const lgd_grad_tensor* tensors_host, int n_tensors, int norm_type, void* ws, float* norm_out, void* stream) {
+    return lgd::norm_call(tensors_host, n_tensors, norm_type, false, 0.f, ws, norm_out, stream);
+}
+
+int lgd_grad_clip(const lgd_grad_tensor* tensors_host, int n_tensors, int norm_type, float max_norm, void* ws, float* norm_out, void* stream) {
+    return lgd::norm_call(tensors_host, n_tensors, norm_type, true, max_norm, ws, norm_out, stream);
+}
+
+}  // extern "C"

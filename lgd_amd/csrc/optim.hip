@@ -9,7 +9,9 @@
 //   d   <- g + wd p
 //   buf <- mu buf + d                       (a zero-initialised buffer reproduces torch's first step, buf = d, exactly)
 //   p   <- p - lr buf
-#include "common.h"
+// or, clipping by NORM (lgd_sgd_norm_step): the gradients of every optimizer are one vector, g <- c g with c = min(1, max_norm / (norm + 1e-6)) of that
+// optimizer's norm; two launches more: partial sums over the same table (reads g once more) and one workgroup per optimizer that joins them.
+#include "grad_norm.h"
 
 #pragma clang fp contract(off)   // mu * buf + d keeps torch's two roundings (mul_ then add_); the fma calls below are explicit
 
@@ -23,8 +25,15 @@ constexpr int kSgdChunk = 4096;  // elements per workgroup: 256 threads x 4 floa
 // the accesses stay dwordx4 (the compiler emits them for this type); round 2 sent such tensors down the scalar path.
 typedef float sgd_f4u __attribute__((ext_vector_type(4), aligned(4)));
 
-template <bool VEC>
+// by value: the clamped gradient, NaN stays NaN (as torch.clamp); by norm: `clip` is the optimizer's factor
+template <bool NORM> __device__ __forceinline__ float sgd_clipped(float g, float clip) {
+    if (NORM) return g * clip;
+    return g < -clip ? -clip : (g > clip ? clip : g);
+}
+
+template <bool VEC, bool NORM>
 __device__ __forceinline__ void sgd_chunk(const lgd_sgd_tensor& t, long long base, float clip) {
+    const bool write_g = !NORM || clip != 1.f;   // a factor of 1 leaves the gradients as they are
     const float lr = t.lr, wd = t.wd, mu = t.mu;
     if constexpr (VEC) {
         float4 p[4], g[4], m[4];
@@ -46,14 +55,14 @@ __device__ __forceinline__ void sgd_chunk(const lgd_sgd_tensor& t, long long bas
             float* pp = &p[k].x; float* gg = &g[k].x; float* mm = &m[k].x;
             #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float c = gg[j] < -clip ? -clip : (gg[j] > clip ? clip : gg[j]);   // NaN stays NaN, as torch.clamp
+                const float c = sgd_clipped<NORM>(gg[j], clip);
                 const float d = __builtin_fmaf(wd, pp[j], c);
                 const float b = mu * mm[j] + d;
                 gg[j] = c; mm[j] = b; pp[j] = __builtin_fmaf(-lr, b, pp[j]);
             }
             *reinterpret_cast<float4*>(t.p + i) = p[k];
             sgd_f4u go; go.x = g[k].x; go.y = g[k].y; go.z = g[k].z; go.w = g[k].w;
-            *reinterpret_cast<sgd_f4u*>(t.g + i) = go;
+            if (write_g) *reinterpret_cast<sgd_f4u*>(t.g + i) = go;
             *reinterpret_cast<float4*>(t.m + i) = m[k];
         }
     }
@@ -63,28 +72,84 @@ __device__ __forceinline__ void sgd_chunk(const lgd_sgd_tensor& t, long long bas
     long long i0 = base;
     if constexpr (VEC) i0 = end == t.n ? (t.n & ~3LL) : end;   // only the last chunk has a tail
     for (long long i = i0 + threadIdx.x; i < end; i += 256) {
-        const float gi = t.g[i];
-        const float c = gi < -clip ? -clip : (gi > clip ? clip : gi);
+        const float c = sgd_clipped<NORM>(t.g[i], clip);
         const float d = __builtin_fmaf(wd, t.p[i], c);
         const float b = mu * t.m[i] + d;
-        t.g[i] = c; t.m[i] = b; t.p[i] = __builtin_fmaf(-lr, b, t.p[i]);
+        if (write_g) t.g[i] = c;
+        t.m[i] = b; t.p[i] = __builtin_fmaf(-lr, b, t.p[i]);
     }
 }
 
-__global__ __launch_bounds__(256) void sgd_clip_kernel(const lgd_sgd_tensor* __restrict__ tab, const int32_t* __restrict__ blk_off,
-                                                        int nt, float clip) {
-    // the tensor this workgroup works on: last i with blk_off[i] <= blockIdx.x (wave-uniform: scalar loads)
-    int lo = 0, hi = nt;
+// the tensor of a block: last i in [lo, hi) with blk_off[i] <= blk (wave-uniform: scalar loads)
+__device__ __forceinline__ int sgd_tensor_of(const int32_t* __restrict__ blk_off, int lo, int hi, int blk) {
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (blk_off[mid] <= (int)blockIdx.x) lo = mid; else hi = mid;
+        if (blk_off[mid] <= blk) lo = mid; else hi = mid;
     }
+    return lo;
+}
+
+template <bool NORM>
+__global__ __launch_bounds__(256) void sgd_clip_kernel(const lgd_sgd_tensor* __restrict__ tab, const int32_t* __restrict__ blk_off,
+                                                        int nt, float clip, const float* __restrict__ coef) {
+    const int lo = sgd_tensor_of(blk_off, 0, nt, (int)blockIdx.x);
     const lgd_sgd_tensor t = tab[lo];
     const long long base = (long long)((int)blockIdx.x - blk_off[lo]) * kSgdChunk;
     if (base >= t.n) return;
     const bool vec = ((reinterpret_cast<uintptr_t>(t.p) | reinterpret_cast<uintptr_t>(t.m)) & 15) == 0 && (reinterpret_cast<uintptr_t>(t.g) & 3) == 0;
-    if (vec) sgd_chunk<true>(t, base, clip);
-    else sgd_chunk<false>(t, base, clip);
+    if (NORM) clip = coef[t.reserved];
+    if (vec) sgd_chunk<true, NORM>(t, base, clip);
+    else sgd_chunk<false, NORM>(t, base, clip);
+}
+
+constexpr int kSgdNormGrid = 512;   // workgroups per optimizer: one partial word each
+struct SgdGroups {
+    int tensor[LGD_MAX_SGD_GROUPS + 1];   // borders in the table
+    int blk[LGD_MAX_SGD_GROUPS + 1];      // and in its blocks
+};
+
+// partial norms of the gradients of group blockIdx.y: each workgroup an equal contiguous run of the group's blocks
+template <int NT>
+__global__ __launch_bounds__(256) void sgd_norm_kernel(const lgd_sgd_tensor* __restrict__ tab, const int32_t* __restrict__ blk_off, SgdGroups g,
+                                                       double* __restrict__ part) {
+    __shared__ double sh[4];
+    const int k = blockIdx.y, nb = g.blk[k + 1] - g.blk[k];
+    const int c1 = g.blk[k] + (int)((long long)nb * (blockIdx.x + 1) / kSgdNormGrid);
+    int c = g.blk[k] + (int)((long long)nb * blockIdx.x / kSgdNormGrid);
+    NormAcc<NT> acc;
+    if (c < c1) {
+        int i = sgd_tensor_of(blk_off, g.tensor[k], g.tensor[k + 1], c);
+        while (c < c1) {
+            const int last = min(c1, blk_off[i + 1]);
+            const long long first = (long long)(c - blk_off[i]) * kSgdChunk, left = tab[i].n - first, want = (long long)(last - c) * kSgdChunk;
+            // a run of blocks of one tensor is contiguous: at most 2^30 elements at once
+            for (long long o = 0; o < want && o < left; o += 1 << 30)
+                norm_chunk<NT, float, 8>(tab[i].g + first + o, (int)min(min(want, left) - o, 1LL << 30), acc);
+            c = last; ++i;
+        }
+    }
+    acc = norm_block<NT>(acc, sh);
+    if (threadIdx.x == 0) part[k * kSgdNormGrid + blockIdx.x] = acc.word();
+}
+
+// one workgroup per group: its norm and its factor
+template <int NT>
+__global__ __launch_bounds__(256) void sgd_coef_kernel(const double* __restrict__ part, float max_norm, float* __restrict__ norms, float* __restrict__ coef) {
+    __shared__ double sh[4];
+    const float v = norm_total<NT>(part + blockIdx.x * kSgdNormGrid, kSgdNormGrid, sh);
+    if (threadIdx.x == 0) { norms[blockIdx.x] = v; coef[blockIdx.x] = norm_coef(v, max_norm); }
+}
+
+template <int NT>
+static int sgd_norm_run(const lgd_sgd_tensor* table, const int32_t* blk_off, int n_tensors, int n_blocks, const SgdGroups& g, int n_groups, float max_norm,
+                        void* ws, float* norms, hipStream_t s) {
+    double* part = static_cast<double*>(ws);
+    float* coef = reinterpret_cast<float*>(part + (size_t)n_groups * kSgdNormGrid);
+    LGD_LAUNCH("sgd_norm_kernel", sgd_norm_kernel<NT>, dim3(kSgdNormGrid, (unsigned)n_groups), dim3(256), 0, s, table, blk_off, g, part);
+    LGD_LAUNCH("sgd_coef_kernel", sgd_coef_kernel<NT>, dim3((unsigned)n_groups), dim3(256), 0, s, part, max_norm, norms, coef);
+    if (n_blocks > 0)
+        LGD_LAUNCH("sgd_norm_step_kernel", sgd_clip_kernel<true>, dim3((unsigned)n_blocks), dim3(256), 0, s, table, blk_off, n_tensors, 0.f, coef);
+    return check_launch();
 }
 
 }  // namespace lgd
@@ -95,9 +160,31 @@ int lgd_sgd_chunk_elems(void) { return lgd::kSgdChunk; }
 
 int lgd_sgd_clip_step(const lgd_sgd_tensor* table, const int32_t* blk_off, int n_tensors, int n_blocks, float clip_value, void* stream) {
     if (!table || !blk_off || n_tensors < 1 || n_blocks < 1 || !(clip_value > 0.f)) return LGD_EINVAL;
-    LGD_LAUNCH("sgd_clip_kernel", lgd::sgd_clip_kernel, dim3((unsigned)n_blocks), dim3(256), 0, (hipStream_t)stream, table, blk_off,
-               n_tensors, clip_value);
+    LGD_LAUNCH("sgd_clip_kernel", lgd::sgd_clip_kernel<false>, dim3((unsigned)n_blocks), dim3(256), 0, (hipStream_t)stream, table, blk_off,
+               n_tensors, clip_value, (const float*)nullptr);
     return lgd::check_launch();
+}
+
+size_t lgd_sgd_norm_ws_bytes(int n_groups) {
+    return n_groups < 1 ? 0 : (size_t)n_groups * (lgd::kSgdNormGrid * sizeof(double) + sizeof(float));
+}
+
+int lgd_sgd_norm_step(const lgd_sgd_tensor* table, const int32_t* blk_off, int n_tensors, int n_blocks, const int32_t* group_off_host,
+                      const int32_t* group_blk_host, int n_groups, int norm_type, float max_norm, void* ws, float* norms_out, void* stream) {
+    if (!table || !blk_off || n_tensors < 1 || n_blocks < 0 || !group_off_host || !group_blk_host || n_groups < 1 || n_groups > LGD_MAX_SGD_GROUPS ||
+        !(max_norm >= 0.f) || !ws || !norms_out)
+        return LGD_EINVAL;
+    lgd::SgdGroups g = {};
+    for (int k = 0; k <= n_groups; ++k) {
+        g.tensor[k] = group_off_host[k]; g.blk[k] = group_blk_host[k];
+        if (k > 0 && (g.tensor[k] < g.tensor[k - 1] || g.blk[k] < g.blk[k - 1] || (g.tensor[k] == g.tensor[k - 1] && g.blk[k] != g.blk[k - 1]))) return LGD_EINVAL;
+    }
+    if (g.tensor[0] != 0 || g.blk[0] != 0 || g.tensor[n_groups] != n_tensors || g.blk[n_groups] != n_blocks) return LGD_EINVAL;
+    hipStream_t s = (hipStream_t)stream;
+    if (norm_type == LGD_NORM_2) return lgd::sgd_norm_run<LGD_NORM_2>(table, blk_off, n_tensors, n_blocks, g, n_groups, max_norm, ws, norms_out, s);
+    if (norm_type == LGD_NORM_1) return lgd::sgd_norm_run<LGD_NORM_1>(table, blk_off, n_tensors, n_blocks, g, n_groups, max_norm, ws, norms_out, s);
+    if (norm_type == LGD_NORM_INF) return lgd::sgd_norm_run<LGD_NORM_INF>(table, blk_off, n_tensors, n_blocks, g, n_groups, max_norm, ws, norms_out, s);
+    return LGD_EINVAL;
 }
 
 }  // extern "C"

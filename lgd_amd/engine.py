@@ -204,8 +204,10 @@ class Trainer:
             self.tuned_gemms = ops.enable_tuned_gemms()  # opt-in here (not an import side effect): lookup-only solution table
             # clip + both SGD updates as one HIP launch (csrc/optim.hip); other optimizers / clip types: torch's multi-tensor path
             if self.fused_sgd_enabled and optim.supported([self.stu_optimizer, self.tea_optimizer], self.clip):
+                by_norm = self.clip.ENABLED and self.clip.CLIP_TYPE == "full_model"
                 self._fused_sgd = optim.FusedClipSGD([self.stu_optimizer, self.tea_optimizer],
-                                                     self.clip.CLIP_VALUE if self.clip.ENABLED else None)
+                                                     self.clip.CLIP_VALUE if self.clip.ENABLED and not by_norm else None,
+                                                     clip_norm=self.clip.CLIP_VALUE if by_norm else None, norm_type=self.clip.NORM_TYPE)
         else:
             self.tuned_gemms = False
 
@@ -283,7 +285,17 @@ class Trainer:
 
     def _clip(self):
         """detectron2 maybe_add_gradient_clipping: per PARAMETER, CLIP_TYPE 'value' (default, CLIP_VALUE 1.0) = element-wise
-        clamp, 'norm' = clip_grad_norm_ of each parameter on its own [d2-memory]; multi-tensor forms, no host sync."""
+        clamp, 'norm' = clip_grad_norm_ of each parameter on its own [d2-memory]; multi-tensor forms, no host sync.  'full_model' = by the
+        norm of each optimizer's whole gradient (optim.clip_grad_norm_ on the GPU, torch's on the CPU)."""
+        if self.clip.CLIP_TYPE == "full_model":
+            for o in (self.stu_optimizer, self.tea_optimizer):
+                params = [p for g in o.param_groups for p in g["params"] if p.grad is not None]
+                if params and params[0].is_cuda:
+                    from . import optim
+                    optim.clip_grad_norm_(params, self.clip.CLIP_VALUE, self.clip.NORM_TYPE)
+                else:
+                    torch.nn.utils.clip_grad_norm_(params, float(self.clip.CLIP_VALUE), float(self.clip.NORM_TYPE))
+            return
         grads = [p.grad for g in self.stu_optimizer.param_groups + self.tea_optimizer.param_groups
                  for p in g["params"] if p.grad is not None]
         if not grads:

@@ -5,6 +5,7 @@ logic stays testable) but any kernel call raises LgdHipError when the library or
 GPU is missing -- the product path must fail loudly rather than silently compute
 elsewhere.
 """
+import contextlib
 import ctypes
 import os
 
@@ -13,7 +14,7 @@ import torch
 _LIB_PATH = os.environ.get("LGD_HIP_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "liblgd_hip.so")   # LGD_HIP_LIB: a lab build
 _lib = None
 
-ABI_VERSION = 26
+ABI_VERSION = 27
 
 c_fp = ctypes.c_void_p
 c_i = ctypes.c_int
@@ -130,6 +131,14 @@ SIGNATURES = {
     "lgd_dcn_col2im": (c_i, [c_fp, c_fp, c_fp, c_fp, c_i, c_i, c_i, c_i, c_i, c_i, c_i, c_fp, c_fp, c_fp, c_fp, c_fp]),
     "lgd_sgd_chunk_elems": (c_i, []),
     "lgd_sgd_clip_step": (c_i, [c_fp, c_fp, c_i, c_i, c_f, c_fp]),
+    "lgd_grad_norm_ws_bytes": (c_sz, [c_i]),
+    "lgd_grad_norm": (c_i, [c_fp, c_i, c_i, c_fp, c_fp, c_fp]),
+    "lgd_grad_clip": (c_i, [c_fp, c_i, c_i, c_f, c_fp, c_fp, c_fp]),
+    "lgd_sgd_norm_ws_bytes": (c_sz, [c_i]),
+    "lgd_sgd_norm_step": (c_i, [c_fp, c_fp, c_i, c_i, c_fp, c_fp, c_i, c_i, c_f, c_fp, c_fp, c_fp]),
+    "lgd_gn_act_ws_bytes": (c_sz, [c_fp, c_i, c_i, c_i, c_i, c_i, c_i]),
+    "lgd_gn_act_fwd": (c_i, [c_fp, c_fp, c_i, c_i, c_i, c_i, c_i, c_fp, c_fp, c_i, ctypes.c_double, c_i, c_fp, c_fp, c_fp, c_fp]),
+    "lgd_gn_act_bwd": (c_i, [c_fp, c_fp, c_fp, c_i, c_i, c_i, c_i, c_i, c_fp, c_fp, c_i, c_i, c_fp, c_fp, c_fp, c_fp, c_fp, c_fp]),
     "lgd_timing_enable": (c_i, [c_i]),
     "lgd_timing_collect": (c_i, [ctypes.c_char_p, c_sz, c_fp, c_fp, c_i]),
     "lgd_timing_collect_ex": (c_i, [ctypes.c_char_p, c_sz, c_fp, c_fp, c_fp, c_fp, c_i]),
@@ -143,6 +152,15 @@ class GemmProblem(ctypes.Structure):
                 ("M", ctypes.c_int32), ("N", ctypes.c_int32), ("K", ctypes.c_int32), ("reserved0", ctypes.c_int32),
                 ("sa_m", ctypes.c_int64), ("sa_k", ctypes.c_int64), ("sb_n", ctypes.c_int64), ("sb_k", ctypes.c_int64),
                 ("sc_m", ctypes.c_int64), ("sc_n", ctypes.c_int64), ("alpha", ctypes.c_float), ("reserved1", ctypes.c_int32)]
+
+
+class GradTensor(ctypes.Structure):
+    """mirror of `lgd_grad_tensor` (include/lgd_hip.h)."""
+    _fields_ = [("p", c_fp), ("n", ctypes.c_int64), ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+# element types of the entry points that take more than fp32 (LGD_F32 / LGD_BF16 / LGD_F16)
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 class LgdHipError(RuntimeError):
@@ -196,6 +214,14 @@ def stream_ptr():
     """the current HIP stream of the current device as a void* (the raw getter: torch.cuda.current_stream() builds a Stream object
     and resolves the device index in Python, ~9 us per call x ~300 calls per step)."""
     return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def device_guard(device):
+    """context that makes `device` the current one (stream_ptr() and the launches follow it); free when it already is."""
+    return _SAME_DEVICE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def ptr(t):

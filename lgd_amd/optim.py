@@ -1,4 +1,5 @@
-"""Gradient clipping + the two SGD updates of the distillation step as ONE HIP launch (csrc/optim.hip).
+"""Gradient norms and clipping over many tensors, and gradient clipping + the two SGD updates of the distillation step as ONE HIP launch
+(csrc/grad_norm.hip, csrc/optim.hip).
 
 [ref: train.py:200-204 -- `stu_optimizer.step(); tea_optimizer.step()`; utils/build.py:494-529 -- torch.optim.SGD with momentum and
 weight decay, wrapped by detectron2's per-parameter gradient clipping (CLIP_TYPE "value").]
@@ -20,11 +21,116 @@ _TENSOR_DT = np.dtype([("p", "<u8"), ("g", "<u8"), ("m", "<u8"), ("n", "<i8"), (
                        ("reserved", "<i4")])  # mirror of lgd_sgd_tensor (include/lgd_hip.h), 48 bytes
 assert _TENSOR_DT.itemsize == 48
 
+_GRAD_DT = np.dtype([("p", "<u8"), ("n", "<i8"), ("dtype", "<i4"), ("reserved", "<i4")])   # mirror of lgd_grad_tensor, 24 bytes
+assert _GRAD_DT.itemsize == ctypes.sizeof(hip.GradTensor) == 24
+
+_NORMS = {2.0: 0, 1.0: 1, float("inf"): 2}   # LGD_NORM_*
+
+
+def _norm_code(norm_type):
+    code = _NORMS.get(float(norm_type))
+    if code is None:
+        raise hip.LgdHipError("norm_type %r: one of 1, 2, inf" % (norm_type,))
+    return code
+
+
+def _dense(t):
+    """whether t's elements fill one contiguous run of memory, in whatever order (channels-last filters do)"""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if st != want:
+            return False
+        want *= n
+    return True
+
+
+def _grad_records(tensors):
+    """-> (records, dense tensors, device): every tensor as the kernels take it.  A tensor that is not one run of memory is replaced by a
+    contiguous copy."""
+    device = tensors[0].device
+    for t in tensors:
+        if t.layout is not torch.strided or t.dtype not in hip.DTYPES or t.device != device:
+            raise hip.LgdHipError("gradient norms take strided fp32, bf16 or fp16 tensors on one device, got %s %s on %s (the first is on %s)"
+                                  % (t.layout, t.dtype, t.device, device))
+    flat = [t if _dense(t) else t.contiguous() for t in tensors]
+    n = len(flat)
+    rec = np.zeros(n, dtype=_GRAD_DT)
+    rec["p"] = np.fromiter(map(torch.Tensor.data_ptr, flat), dtype=np.uint64, count=n)
+    rec["n"] = np.fromiter(map(torch.Tensor.numel, flat), dtype=np.int64, count=n)
+    rec["dtype"] = [hip.DTYPES[t.dtype] for t in flat]
+    return rec, flat, device
+
+
+@torch.no_grad()
+def grad_norm(tensors, norm_type=2.0):
+    """norm over every element of every tensor (fp32 / bf16 / fp16, mixed) as ONE vector -> 0-dim fp32 tensor on their device, no host sync:
+    norm_type 2, 1 or inf.  Sums are 64-bit and run in a fixed order.  A NaN anywhere gives NaN.  No tensors: 0 on the CPU."""
+    code = _norm_code(norm_type)
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    if not tensors:
+        return torch.tensor(0.0)
+    rec, flat, device = _grad_records(tensors)
+    hip.require_gpu(tensors[0])
+    lib = hip.load()
+    with hip.device_guard(device):
+        out = torch.empty((), dtype=torch.float32, device=device)
+        ws = torch.empty(lib.lgd_grad_norm_ws_bytes(len(rec)), dtype=torch.uint8, device=device)
+        hip.check(lib.lgd_grad_norm(ctypes.c_void_p(rec.ctypes.data), len(rec), code, hip.ptr(ws), hip.ptr(out), hip.stream_ptr()), "lgd_grad_norm")
+    return out
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0):
+    """clip the gradients of `parameters` (a tensor or an iterable; those without a gradient are skipped) IN PLACE by the norm of all of them
+    taken together, torch.nn.utils.clip_grad_norm_'s arithmetic: g *= min(1, max_norm / (norm + 1e-6)).  -> the norm before clipping (0-dim
+    fp32 on the device).  No host sync, two launches over all the tensors; nothing is written where nothing has to be clipped.  A norm that is
+    not finite reaches the gradients as it does in torch (NaN everywhere, or 0 and NaN).  The gradients must not share memory."""
+    code = _norm_code(norm_type)
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise hip.LgdHipError("max_norm must not be negative, got %r" % max_norm)
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.tensor(0.0)
+    rec, flat, device = _grad_records(grads)
+    _refuse_shared(rec, grads, flat)
+    hip.require_gpu(grads[0])
+    lib = hip.load()
+    with hip.device_guard(device):
+        out = torch.empty((), dtype=torch.float32, device=device)
+        ws = torch.empty(lib.lgd_grad_norm_ws_bytes(len(rec)), dtype=torch.uint8, device=device)
+        hip.check(lib.lgd_grad_clip(ctypes.c_void_p(rec.ctypes.data), len(rec), code, ctypes.c_float(max_norm), hip.ptr(ws), hip.ptr(out),
+                                    hip.stream_ptr()), "lgd_grad_clip")
+        for g, f in zip(grads, flat):
+            if f is not g:
+                g.copy_(f)
+    torch.autograd.graph.increment_version(grads)   # written through raw pointers
+    return out
+
+
+def _refuse_shared(rec, grads, flat):
+    """in-place scaling needs every element once: a gradient listed twice, an expanded one, or views that overlap are refused"""
+    size = np.where(rec["dtype"] == 0, 4, 2)
+    live = rec["n"] > 0
+    p, e = rec["p"][live].astype(np.int64), (rec["p"].astype(np.int64) + rec["n"] * size)[live]
+    order = np.argsort(p, kind="stable")
+    if len(p) > 1 and bool((e[order][:-1] > p[order][1:]).any()):
+        raise hip.LgdHipError("two of the gradients share memory: each element can be clipped once")
+    strided = [g for g, f in zip(grads, flat) if f is not g]
+    if any(st == 0 and n > 1 for g in strided for st, n in zip(g.stride(), g.shape)) or len({g.data_ptr() for g in strided}) != len(strided):
+        raise hip.LgdHipError("a gradient that is expanded, or listed twice, cannot be clipped in place")
+
 
 def supported(optimizers, clip):
     """the fused step covers what the reference's configs use: SGD (dampening 0, no Nesterov, not maximize) on fp32 CUDA parameters,
-    gradient clipping off or CLIP_TYPE 'value'; anything else stays on torch's own multi-tensor path."""
-    if clip.ENABLED and clip.CLIP_TYPE != "value":
+    gradient clipping off, CLIP_TYPE 'value', or 'full_model' (by the norm of each optimizer's whole gradient; NORM_TYPE 1, 2 or inf); anything
+    else stays on torch's own multi-tensor path."""
+    if clip.ENABLED and clip.CLIP_TYPE not in ("value", "full_model"):
+        return False
+    if clip.ENABLED and clip.CLIP_TYPE == "full_model" and float(clip.NORM_TYPE) not in _NORMS:
         return False
     for o in optimizers:
         if type(o) is not torch.optim.SGD:
@@ -39,12 +145,18 @@ def supported(optimizers, clip):
 
 
 class FusedClipSGD:
-    """step() = clip + update of every parameter that has a gradient, over all the given torch.optim.SGD objects."""
+    """step() = clip + update of every parameter that has a gradient, over all the given torch.optim.SGD objects.
+    clip_value: element-wise clamp.  clip_norm: the gradients of EACH optimizer are scaled by min(1, clip_norm / (norm + 1e-6)) of their own
+    norm (norm_type 2, 1 or inf) -- torch.nn.utils.clip_grad_norm_ per optimizer, then its step(); `total_norms` then holds the norms
+    before clipping of the last step (one fp32 per optimizer, on the device).  Neither: no clipping.  The clipped gradients are written back."""
     SLOTS = 8  # pinned staging tables in flight (a slot is reused SLOTS steps later, after its upload event has completed)
 
-    def __init__(self, optimizers, clip_value=None):
+    def __init__(self, optimizers, clip_value=None, clip_norm=None, norm_type=2.0):
         self.optimizers = list(optimizers)
+        if clip_value is not None and clip_norm is not None:
+            raise hip.LgdHipError("clip by value or by norm, not both")
         self.clip_value = float("inf") if clip_value is None else float(clip_value)
+        self.clip_norm, self.norm_type, self.total_norms = clip_norm, norm_type, None
         self.params, self.owner = [], []
         for k, o in enumerate(self.optimizers):
             for gi, g in enumerate(o.param_groups):
@@ -52,6 +164,10 @@ class FusedClipSGD:
                     self.params.append(p)
                     self.owner.append((k, gi))
         n = len(self.params)
+        if clip_norm is not None:
+            _norm_code(norm_type)
+            if len({id(p) for p in self.params}) != n or not 1 <= len(self.optimizers) <= 16:
+                raise hip.LgdHipError("clipping by norm takes 1 to 16 optimizers (LGD_MAX_SGD_GROUPS) that share no parameter")
         self._numel = np.array([p.numel() for p in self.params], dtype=np.int64)
         self._m_ptr = np.zeros(n, dtype=np.uint64)
         self._m_ref = [None] * n   # the buffer each cached pointer belongs to
@@ -97,9 +213,16 @@ class FusedClipSGD:
             self.chunk = int(lib.lgd_sgd_chunk_elems())
         grads = [p.grad for p in self.params]
         idx = [i for i, g in enumerate(grads) if g is not None]
+        by_norm = self.clip_norm is not None
+        if by_norm and not float(self.clip_norm) >= 0:
+            raise hip.LgdHipError("clip_norm must not be negative, got %r" % (self.clip_norm,))
         if not idx:
+            if by_norm:
+                self.total_norms = torch.zeros(len(self.optimizers), device=self.params[0].device if self.params else None)
             return
         hip.require_gpu(grads[idx[0]])
+        if by_norm and torch.cuda.is_current_stream_capturing():
+            raise hip.LgdHipError("the fused step uploads its table from host memory that later steps reuse: it cannot be captured into a graph")
         if idx != self._checked_idx:   # layout checks once per set of parameters that receive gradients (autograd hands out the
             for i in idx:              # same kind of tensor every step; the checks cost ~0.12 ms of the ~0.4 ms this call takes)
                 g = grads[i]
@@ -132,7 +255,8 @@ class FusedClipSGD:
             hyper[key] = (float(g["lr"]), float(g["weight_decay"]), float(g["momentum"]))
         hy = np.array([hyper[key] for key in self._grp[ii].tolist()], dtype=np.float32)
         tab["lr"], tab["wd"], tab["mu"] = hy[:, 0], hy[:, 1], hy[:, 2]
-        tab["reserved"] = 0
+        owner = self._grp[ii] // 4096
+        tab["reserved"] = owner if by_norm else 0
         blk[0] = 0
         blk[1:] = np.cumsum((self._numel[ii] + self.chunk - 1) // self.chunk)
         n_blocks = int(blk[k])
@@ -144,8 +268,19 @@ class FusedClipSGD:
             ev = self._events[s] = torch.cuda.Event()
         ev.record()
         base = dev.data_ptr()
-        hip.check(lib.lgd_sgd_clip_step(ctypes.c_void_p(base), ctypes.c_void_p(base + 48 * k), k, n_blocks,
-                                        ctypes.c_float(self.clip_value), hip.stream_ptr()), "lgd_sgd_clip_step")
+        if by_norm:
+            ng = len(self.optimizers)
+            border = np.searchsorted(owner, np.arange(ng + 1)).astype(np.int32)   # the table is ordered by optimizer
+            border_blk = blk[border]
+            norms = torch.empty(ng, dtype=torch.float32, device=device)
+            ws = torch.empty(lib.lgd_sgd_norm_ws_bytes(ng), dtype=torch.uint8, device=device)
+            hip.check(lib.lgd_sgd_norm_step(ctypes.c_void_p(base), ctypes.c_void_p(base + 48 * k), k, n_blocks, ctypes.c_void_p(border.ctypes.data),
+                                            ctypes.c_void_p(border_blk.ctypes.data), ng, _norm_code(self.norm_type), ctypes.c_float(float(self.clip_norm)),
+                                            hip.ptr(ws), hip.ptr(norms), hip.stream_ptr()), "lgd_sgd_norm_step")
+            self.total_norms = norms
+        else:
+            hip.check(lib.lgd_sgd_clip_step(ctypes.c_void_p(base), ctypes.c_void_p(base + 48 * k), k, n_blocks,
+                                            ctypes.c_float(self.clip_value), hip.stream_ptr()), "lgd_sgd_clip_step")
         # the kernel wrote p, g and the momentum buffers through raw pointers: tell autograd's version counters, which the fold
         # caches (ConvBN._frozen_fold, FrozenBatchNorm2d.scale_shift) key on and the saved-tensor check reads
         torch.autograd.graph.increment_version([params[i] for i in idx] + [grads[i] for i in idx] + [self._m_ref[i] for i in idx])
