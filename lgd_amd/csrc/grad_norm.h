@@ -35,17 +35,15 @@ template <typename T> __device__ __forceinline__ int norm_head(const T* p, int c
 }
 
 // `count` contiguous elements by a workgroup of 256 threads: 16-byte loads between an unaligned head and tail, U of them in flight
-template <int NT, typename T, int U>
+template <int NT, typename T, int U, bool STREAM>
 __device__ __forceinline__ void norm_chunk(const T* __restrict__ p, int count, NormAcc<NT>& acc) {
     constexpr int V = Vec16<T>::V;
     const int t = threadIdx.x, head = norm_head(p, count), nv = (count - head) / V, tail = head + nv * V;
-    if (t < head) acc.add((float)p[t]);
-    if (t < count - tail) acc.add((float)p[tail + t]);
-    const lgd_u32x4* __restrict__ q = reinterpret_cast<const lgd_u32x4*>(p + head);
+    const T* q = p + head;
     for (int i0 = t; i0 < nv; i0 += 256 * U) {
         lgd_u32x4 v[U];
         #pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = i0 + u * 256 < nv ? q[i0 + u * 256] : (lgd_u32x4){0, 0, 0, 0};   // zeros add nothing to any of the norms
+        for (int u = 0; u < U; ++u) v[u] = i0 + u * 256 < nv ? vec16_load<STREAM>(q + (size_t)(i0 + u * 256) * V) : (lgd_u32x4){0, 0, 0, 0};   // zeros add nothing to any of the norms
         #pragma unroll
         for (int u = 0; u < U; ++u) {
             float f[V];
@@ -54,7 +52,33 @@ __device__ __forceinline__ void norm_chunk(const T* __restrict__ p, int count, N
             for (int i = 0; i < V; ++i) acc.add(f[i]);
         }
     }
+    if (t < head) acc.add((float)glob_load(p + t));
+    if (t < count - tail) acc.add((float)glob_load(p + tail + t));
 }
+
+// Which tensor holds block c: the last one whose first block is not behind c.  Every lane holds the first blocks of its tensors (lane, lane + 64, ...:
+// ascending), a ballot counts them -- one load latency per kernel instead of a chain of dependent ones per block; lists longer than 64 K load the rest.
+template <int K, typename First>
+struct TensorFinder {
+    First first;   // first(i): first block of tensor i
+    int lo, n, b0[K];
+    __device__ __forceinline__ TensorFinder(First f, int lo_, int hi) : first(f), lo(lo_), n(hi - lo_) {
+        const int lane = threadIdx.x & 63;
+        #pragma unroll
+        for (int k = 0; k < K; ++k) b0[k] = k * 64 + lane < n ? first(lo + k * 64 + lane) : 0x7fffffff;
+    }
+    __device__ __forceinline__ int find(int c) const {
+        int i = lo - 1;
+        #pragma unroll
+        for (int k = 0; k < K; ++k) i += __popcll(__ballot(b0[k] <= c));
+        for (int k = K; k * 64 < n; ++k) {
+            const int j = k * 64 + (int)(threadIdx.x & 63);
+            i += __popcll(__ballot((j < n ? first(lo + j) : 0x7fffffff) <= c));
+        }
+        return __builtin_amdgcn_readfirstlane(i);
+    }
+};
+template <int K, typename First> __device__ __forceinline__ TensorFinder<K, First> tensor_finder(First f, int lo, int hi) { return TensorFinder<K, First>(f, lo, hi); }
 
 // the workgroup's accumulators as one, in every thread (sh: 4 words; barriers inside)
 template <int NT>

@@ -25,6 +25,17 @@ constexpr int kSgdChunk = 4096;  // elements per workgroup: 256 threads x 4 floa
 // the accesses stay dwordx4 (the compiler emits them for this type); round 2 sent such tensors down the scalar path.
 typedef float sgd_f4u __attribute__((ext_vector_type(4), aligned(4)));
 
+// global accesses (the pointers come out of a table: generic to the compiler otherwise), streaming: nothing of a step's six
+// transfers is used again in it (37 M parameters, clipped by norm: 167 us a step, 198 - 205 with plain loads, plain stores or both)
+typedef __attribute__((address_space(1))) const sgd_f4u* sgd_gptr;
+typedef __attribute__((address_space(1))) sgd_f4u* sgd_gptr_rw;
+typedef __attribute__((address_space(1))) const lgd_vf4* sgd_gptr4;
+typedef __attribute__((address_space(1))) lgd_vf4* sgd_gptr4_rw;
+__device__ __forceinline__ float4 sgd_load4(const float* p) { const lgd_vf4 v = __builtin_nontemporal_load((sgd_gptr4)p); return make_float4(v.x, v.y, v.z, v.w); }
+__device__ __forceinline__ sgd_f4u sgd_loadu(const float* p) { return __builtin_nontemporal_load((sgd_gptr)p); }
+__device__ __forceinline__ void sgd_store4(float* p, const float4& f) { const lgd_vf4 v = {f.x, f.y, f.z, f.w}; __builtin_nontemporal_store(v, (sgd_gptr4_rw)p); }
+__device__ __forceinline__ void sgd_storeu(float* p, const sgd_f4u& v) { __builtin_nontemporal_store(v, (sgd_gptr_rw)p); }
+
 // by value: the clamped gradient, NaN stays NaN (as torch.clamp); by norm: `clip` is the optimizer's factor
 template <bool NORM> __device__ __forceinline__ float sgd_clipped(float g, float clip) {
     if (NORM) return g * clip;
@@ -43,8 +54,8 @@ __device__ __forceinline__ void sgd_chunk(const lgd_sgd_tensor& t, long long bas
             const long long i = base + (long long)(k * 256 + threadIdx.x) * 4;
             on[k] = i + 3 < t.n;
             if (on[k]) {
-                p[k] = *reinterpret_cast<const float4*>(t.p + i); m[k] = *reinterpret_cast<const float4*>(t.m + i);
-                const sgd_f4u gv = *reinterpret_cast<const sgd_f4u*>(t.g + i);
+                p[k] = sgd_load4(t.p + i); m[k] = sgd_load4(t.m + i);
+                const sgd_f4u gv = sgd_loadu(t.g + i);
                 g[k] = make_float4(gv.x, gv.y, gv.z, gv.w);
             }
         }
@@ -60,10 +71,10 @@ __device__ __forceinline__ void sgd_chunk(const lgd_sgd_tensor& t, long long bas
                 const float b = mu * mm[j] + d;
                 gg[j] = c; mm[j] = b; pp[j] = __builtin_fmaf(-lr, b, pp[j]);
             }
-            *reinterpret_cast<float4*>(t.p + i) = p[k];
+            sgd_store4(t.p + i, p[k]);
             sgd_f4u go; go.x = g[k].x; go.y = g[k].y; go.z = g[k].z; go.w = g[k].w;
-            if (write_g) *reinterpret_cast<sgd_f4u*>(t.g + i) = go;
-            *reinterpret_cast<float4*>(t.m + i) = m[k];
+            if (write_g) sgd_storeu(t.g + i, go);
+            sgd_store4(t.m + i, m[k]);
         }
     }
     // scalar path: parameters / momentum buffers that are not 16-byte aligned (never torch's own allocations), and the < 4-element
@@ -108,25 +119,19 @@ struct SgdGroups {
     int blk[LGD_MAX_SGD_GROUPS + 1];      // and in its blocks
 };
 
-// partial norms of the gradients of group blockIdx.y: each workgroup an equal contiguous run of the group's blocks
+// partial norms of the gradients of group blockIdx.y; its workgroups sweep the group's blocks side by side.  Plain loads: what fits stays in the caches
+// for the update's read
 template <int NT>
 __global__ __launch_bounds__(256) void sgd_norm_kernel(const lgd_sgd_tensor* __restrict__ tab, const int32_t* __restrict__ blk_off, SgdGroups g,
                                                        double* __restrict__ part) {
     __shared__ double sh[4];
-    const int k = blockIdx.y, nb = g.blk[k + 1] - g.blk[k];
-    const int c1 = g.blk[k] + (int)((long long)nb * (blockIdx.x + 1) / kSgdNormGrid);
-    int c = g.blk[k] + (int)((long long)nb * blockIdx.x / kSgdNormGrid);
+    const int k = blockIdx.y;
     NormAcc<NT> acc;
-    if (c < c1) {
-        int i = sgd_tensor_of(blk_off, g.tensor[k], g.tensor[k + 1], c);
-        while (c < c1) {
-            const int last = min(c1, blk_off[i + 1]);
-            const long long first = (long long)(c - blk_off[i]) * kSgdChunk, left = tab[i].n - first, want = (long long)(last - c) * kSgdChunk;
-            // a run of blocks of one tensor is contiguous: at most 2^30 elements at once
-            for (long long o = 0; o < want && o < left; o += 1 << 30)
-                norm_chunk<NT, float, 8>(tab[i].g + first + o, (int)min(min(want, left) - o, 1LL << 30), acc);
-            c = last; ++i;
-        }
+    const auto finder = tensor_finder<6>([&](int i) { return (int)blk_off[i]; }, g.tensor[k], g.tensor[k + 1]);
+    for (int c = g.blk[k] + (int)blockIdx.x; c < g.blk[k + 1]; c += kSgdNormGrid) {
+        const int i = finder.find(c);
+        const long long first = (long long)(c - blk_off[i]) * kSgdChunk, left = tab[i].n - first;
+        norm_chunk<NT, float, 4, false>(tab[i].g + first, (int)(left < kSgdChunk ? left : kSgdChunk), acc);
     }
     acc = norm_block<NT>(acc, sh);
     if (threadIdx.x == 0) part[k * kSgdNormGrid + blockIdx.x] = acc.word();

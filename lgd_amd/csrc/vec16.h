@@ -55,4 +55,21 @@ template <> struct Vec16<_Float16> {
     }
 };
 
+// 16-byte accesses of GLOBAL memory: pointers that come out of a table in memory are generic to the compiler, and a flat access also takes an LDS
+// slot and waits on both counters.  NT: streaming (does not displace what the caches hold)
+typedef __attribute__((address_space(1))) const lgd_u32x4* vec16_gptr;
+typedef __attribute__((address_space(1))) lgd_u32x4* vec16_gptr_rw;
+template <bool NT> __device__ __forceinline__ lgd_u32x4 vec16_load(const void* p) {
+    const vec16_gptr g = (vec16_gptr)p;
+    if constexpr (NT) return __builtin_nontemporal_load(g);
+    else return *g;
+}
+template <bool NT> __device__ __forceinline__ void vec16_store(void* p, const lgd_u32x4& v) {
+    const vec16_gptr_rw g = (vec16_gptr_rw)p;
+    if constexpr (NT) __builtin_nontemporal_store(v, g);
+    else *g = v;
+}
+template <typename T> __device__ __forceinline__ T glob_load(const T* p) { return *(__attribute__((address_space(1))) const T*)p; }
+template <typename T> __device__ __forceinline__ void glob_store(T* p, T v) { *(__attribute__((address_space(1))) T*)p = v; }
+
 }  // namespace lgd

@@ -11,6 +11,7 @@ ops and two optimizers) and ~40 launches over 13 tensor transfers per element; a
 optimizer entry.  Here the host builds one table (three pointers, length, lr / wd / mu per tensor) in pinned memory and launches once.
 """
 import ctypes
+import operator
 
 import numpy as np
 import torch
@@ -25,6 +26,9 @@ _GRAD_DT = np.dtype([("p", "<u8"), ("n", "<i8"), ("dtype", "<i4"), ("reserved", 
 assert _GRAD_DT.itemsize == ctypes.sizeof(hip.GradTensor) == 24
 
 _NORMS = {2.0: 0, 1.0: 1, float("inf"): 2}   # LGD_NORM_*
+
+
+_kind = operator.attrgetter("dtype", "device", "layout")
 
 
 def _norm_code(norm_type):
@@ -49,17 +53,19 @@ def _dense(t):
 def _grad_records(tensors):
     """-> (records, dense tensors, device): every tensor as the kernels take it.  A tensor that is not one run of memory is replaced by a
     contiguous copy."""
+    kinds = set(map(_kind, tensors))   # C-level passes over the list: what a call costs the host is per tensor
     device = tensors[0].device
-    for t in tensors:
-        if t.layout is not torch.strided or t.dtype not in hip.DTYPES or t.device != device:
+    for dtype, dev, layout in kinds:
+        if layout is not torch.strided or dtype not in hip.DTYPES or dev != device:
             raise hip.LgdHipError("gradient norms take strided fp32, bf16 or fp16 tensors on one device, got %s %s on %s (the first is on %s)"
-                                  % (t.layout, t.dtype, t.device, device))
-    flat = [t if _dense(t) else t.contiguous() for t in tensors]
+                                  % (layout, dtype, dev, device))
+    flat = tensors if all(map(torch.Tensor.is_contiguous, tensors)) else [t if _dense(t) else t.contiguous() for t in tensors]
     n = len(flat)
-    rec = np.zeros(n, dtype=_GRAD_DT)
+    rec = np.empty(n, dtype=_GRAD_DT)
     rec["p"] = np.fromiter(map(torch.Tensor.data_ptr, flat), dtype=np.uint64, count=n)
     rec["n"] = np.fromiter(map(torch.Tensor.numel, flat), dtype=np.int64, count=n)
-    rec["dtype"] = [hip.DTYPES[t.dtype] for t in flat]
+    rec["dtype"] = hip.DTYPES[tensors[0].dtype] if len(kinds) == 1 else [hip.DTYPES[t.dtype] for t in flat]
+    rec["reserved"] = 0
     return rec, flat, device
 
 
@@ -104,21 +110,26 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0):
         ws = torch.empty(lib.lgd_grad_norm_ws_bytes(len(rec)), dtype=torch.uint8, device=device)
         hip.check(lib.lgd_grad_clip(ctypes.c_void_p(rec.ctypes.data), len(rec), code, ctypes.c_float(max_norm), hip.ptr(ws), hip.ptr(out),
                                     hip.stream_ptr()), "lgd_grad_clip")
-        for g, f in zip(grads, flat):
-            if f is not g:
-                g.copy_(f)
+        if flat is not grads:
+            for g, f in zip(grads, flat):
+                if f is not g:
+                    g.copy_(f)
     torch.autograd.graph.increment_version(grads)   # written through raw pointers
     return out
 
 
 def _refuse_shared(rec, grads, flat):
     """in-place scaling needs every element once: a gradient listed twice, an expanded one, or views that overlap are refused"""
-    size = np.where(rec["dtype"] == 0, 4, 2)
-    live = rec["n"] > 0
-    p, e = rec["p"][live].astype(np.int64), (rec["p"].astype(np.int64) + rec["n"] * size)[live]
-    order = np.argsort(p, kind="stable")
-    if len(p) > 1 and bool((e[order][:-1] > p[order][1:]).any()):
+    p = rec["p"].astype(np.int64)
+    e = p + rec["n"] * np.where(rec["dtype"] == 0, 4, 2)
+    live = e > p
+    if not live.all():
+        p, e = p[live], e[live]
+    order = np.argsort(p)
+    if bool((e[order][:-1] > p[order][1:]).any()):
         raise hip.LgdHipError("two of the gradients share memory: each element can be clipped once")
+    if flat is grads:
+        return
     strided = [g for g, f in zip(grads, flat) if f is not g]
     if any(st == 0 and n > 1 for g in strided for st, n in zip(g.stride(), g.shape)) or len({g.data_ptr() for g in strided}) != len(strided):
         raise hip.LgdHipError("a gradient that is expanded, or listed twice, cannot be clipped in place")

@@ -65,6 +65,13 @@ def test_gradients_that_share_memory_are_refused():
             optim.clip_grad_norm_([_param(g) for g in grads], 1.0)
 
 
+def test_views_side_by_side_do_not_share():
+    buf = torch.zeros(100)
+    for grads in ([buf[:50], buf[50:]], [buf[60:], buf[:60], buf[5:5], buf[60:60]], [buf[:0], buf]):
+        rec, flat, _ = optim._grad_records(grads)
+        optim._refuse_shared(rec, grads, flat)
+
+
 @pytest.mark.skipif(torch.cuda.is_available(), reason="checks the no-GPU failure mode")
 def test_no_gpu_no_answer():
     for call in (lambda: ops.group_norm_act([_x(1, 6, 2, 2)], 2), lambda: optim.grad_norm([_x(3)]),
