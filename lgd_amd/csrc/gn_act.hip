@@ -13,13 +13,21 @@
 // Precision.  Sums of x and x^2 are fp64 (gfx950 runs fp64 FMA at the rate of unpacked fp32), the statistics stay fp64, and z = x (r gamma) +
 // (beta - mu r gamma) is ONE fp64 FMA per element: the sign a ReLU's gradient hangs on is decided in 64 bits.  Sums of the backward are fp32 over one
 // thread's rows of a chunk (<= a few hundred terms) and its workgroup, fp64 from there on.  Outputs are rounded once (fp32 -> 16 bits).
-#include "vec16.h"
+#include "gn_act.h"
 
 namespace lgd {
 
+#ifndef GA_SLAB
+#define GA_SLAB 1
+#endif
+#ifndef GA_TARGET
+#define GA_TARGET 1024
+#define GA_U 4
+#define GA_UB 2
+#endif
 constexpr int kGaThreads = 256;
-
-enum GaAct { kActNone = 0, kActRelu = 1, kActSilu = 2 };
+constexpr int kGaFusedG = 512;         // groups of a fused call at most (its statistics lie in LDS) ...
+constexpr int kGaFusedRecords = 4096;  // ... and records x groups of a sample (64 KB that every workgroup of the apply kernel reads from the L2)
 
 struct GaArgs {
     const void* x[LGD_MAX_LEVELS];
@@ -27,19 +35,22 @@ struct GaArgs {
     void* out[LGD_MAX_LEVELS];       // fwd: y ; bwd: dx
     int E[LGD_MAX_LEVELS];           // elements per sample, HW * C
     int HW[LGD_MAX_LEVELS];
-    int spc[LGD_MAX_LEVELS];         // super-rows per chunk
-    int K[LGD_MAX_LEVELS];           // chunks per sample
+    int K[LGD_MAX_LEVELS];           // workgroups (chunks) per sample
     int wg0[LGD_MAX_LEVELS + 1];     // first workgroup of the map: B * K per map
     int L, B, C, G, cg;
     int P, PV;                       // super-row: elements, vectors
     int cols, R, nCB;                // vectors of a column block, super-rows a workgroup covers at once, column blocks
-    int W;                           // width of a chunk's record in `part`: G (forward, one column block), C (backward, one column block) or P
+    int whole;                       // column blocks hold whole groups (a single one always does)
+    int W;                           // width of a chunk's record in `part`: whole: G (forward), C (backward); otherwise P
     double eps;
     const void* gamma;               // [C] or null
     const void* beta;
     int ptype;                       // LGD_F32 / LGD_BF16 / LGD_F16
     double* partd;                   // forward [chunk][W][2]
     float* partf;                    // backward [chunk][W][2]
+    float* partg;                    // backward, fused: [chunk][G][2], the channel sums with gamma, by group
+    int fused;                       // the apply kernels reduce the records themselves (no kernel in between)
+    int nparam;                      // fused backward: workgroups in front of the apply kernel's own that make dgamma and dbeta
     double* stats;                   // [L*B*G][2] mean, rstd
     float* bstats;                   // [L*B*G][2] m1, m2
     double* csum;                    // [L*B][C][2] sum g, sum g xh
@@ -52,28 +63,21 @@ template <int ALIGN> struct GaU;
 template <> struct GaU<2> { typedef uint32_t type __attribute__((ext_vector_type(4), aligned(2))); };
 template <> struct GaU<4> { typedef uint32_t type __attribute__((ext_vector_type(4), aligned(4))); };
 template <typename T> __device__ __forceinline__ lgd_u32x4 ga_load(const T* p) { return *reinterpret_cast<const typename GaU<sizeof(T)>::type*>(p); }
-template <typename T> __device__ __forceinline__ void ga_store(T* p, const lgd_u32x4& u) { *reinterpret_cast<typename GaU<sizeof(T)>::type*>(p) = u; }
-
-// gamma / beta in any of the three types; null: the neutral value
-__device__ __forceinline__ float ga_param(const void* p, int type, int c, float none) {
-    if (!p) return none;
-    if (type == LGD_F32) return static_cast<const float*>(p)[c];
-    if (type == LGD_BF16) return (float)static_cast<const __bf16*>(p)[c];
-    return (float)static_cast<const _Float16*>(p)[c];
-}
-__device__ __forceinline__ void ga_param_store(void* p, int type, int c, float v) {
-    if (type == LGD_F32) static_cast<float*>(p)[c] = v;
-    else if (type == LGD_BF16) static_cast<__bf16*>(p)[c] = (__bf16)v;
-    else static_cast<_Float16*>(p)[c] = (_Float16)v;
+template <typename T> __device__ __forceinline__ lgd_u32x4 ga_stream(const T* p) { return __builtin_nontemporal_load(reinterpret_cast<const typename GaU<sizeof(T)>::type*>(p)); }
+template <typename T> __device__ __forceinline__ void ga_store(T* p, const lgd_u32x4& u) {
+    __builtin_nontemporal_store((typename GaU<sizeof(T)>::type)u, reinterpret_cast<typename GaU<sizeof(T)>::type*>(p));
 }
 
-// sigmoid: v_exp_f32 and v_rcp_f32 (one ulp each); z = -inf gives 0, +inf gives 1
-__device__ __forceinline__ float ga_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * z)); }
-
-template <int ACT> __device__ __forceinline__ float ga_act(float z) {
-    if (ACT == kActRelu) return z <= 0.f ? 0.f : z;   // NaN passes, as torch.relu
-    if (ACT == kActSilu) return z * ga_sigmoid(z);
-    return z;
+// the channels and groups of a column block (whole ones only)
+struct GaBlock { int c0, nc, g0, ng; };
+template <int V> __device__ __forceinline__ GaBlock ga_block(const GaArgs& a) {
+    GaBlock q = {0, a.C, 0, a.G};
+    if (a.nCB > 1) {
+        q.c0 = blockIdx.y * a.cols * V;
+        q.nc = min(a.cols * V, a.C - q.c0);
+        q.g0 = q.c0 / a.cg; q.ng = q.nc / a.cg;
+    }
+    return q;
 }
 
 struct GaWhere { int l, b, k; };
@@ -87,39 +91,76 @@ __device__ __forceinline__ GaWhere ga_locate(const GaArgs& a, int w) {
     return q;
 }
 
-// what a thread owns: vector column v of the super-row, super-rows s0 + r, s0 + r + R, ... of the chunk [s0, s1)
-struct GaThread { int v, s, s1, slim, on; };
+// what a thread owns: vector column v of the super-row, super-rows r, r + R, ... of the blocks of U * R super-rows k, k + K, ... of its sample (the
+// sample's workgroups sweep it side by side: a contiguous run for each reads 10 % slower)
+struct GaThread { int v, r, on, send; };   // send: super-rows in which the thread's vector is whole
 template <int V>
-__device__ __forceinline__ GaThread ga_thread(const GaArgs& a, const GaWhere& q) {
+__device__ __forceinline__ GaThread ga_thread(const GaArgs& a, int E) {
     GaThread t;
-    const int r = threadIdx.x / a.cols, col = threadIdx.x % a.cols;
-    t.v = blockIdx.y * a.cols + col;
-    t.on = r < a.R && t.v < a.PV;
-    t.s = q.k * a.spc[q.l] + r;
-    const int NS = (a.E[q.l] + a.P - 1) / a.P;
-    t.s1 = min(NS, (q.k + 1) * a.spc[q.l]);
-    if (!t.on) t.s1 = 0;
-    const int room = a.E[q.l] - (t.v + 1) * V;   // the vector of super-row s is whole iff s * P <= room
-    t.slim = room < 0 ? 0 : room / a.P + 1;
+    t.r = threadIdx.x / a.cols;
+    t.v = blockIdx.y * a.cols + (threadIdx.x - t.r * a.cols);
+    t.on = t.r < a.R && t.v < a.PV;
+    const int room = E - (t.v + 1) * V;   // the vector of super-row s is whole iff s * P <= room
+    t.send = !t.on || room < 0 ? 0 : room / a.P + 1;
     return t;
 }
 
-// every vector of the thread in order, U loads in flight; the (at most one) vector that the sample's end cuts comes last, zero filled.
-// load(e) starts a vector's loads into a register struct, use(regs, e, count) consumes it
-template <int V, int U, typename Regs, typename Load, typename Part, typename Use>
-__device__ __forceinline__ void ga_walk(const GaArgs& a, const GaThread& t, int E, Load load, Part part, Use use) {
-    const int send = min(t.s1, t.slim), step = a.R * a.P;
-    int s = t.s;
-    long e = (long)s * a.P + (long)t.v * V;
-    for (; s + (U - 1) * a.R < send; s += U * a.R, e += (long)U * step) {
-        Regs q[U];
-        #pragma unroll
-        for (int u = 0; u < U; ++u) q[u] = load(e + (long)u * step);
-        #pragma unroll
-        for (int u = 0; u < U; ++u) use(q[u], e + (long)u * step, V);
+// the loads of a thread's first block, when it is whole (kernels that have something to compute first issue them in front of it)
+template <int V, int U, typename Regs> struct GaFirst {
+    Regs v[U];
+    bool have;
+    template <typename Load> __device__ __forceinline__ void issue(const GaArgs& a, const GaWhere& q, const GaThread& t, Load load) {
+        const int s = q.k * U * a.R + t.r;
+        have = t.on && s + (U - 1) * a.R < t.send;
+        if (have) {
+            const unsigned e = (unsigned)s * a.P + t.v * V;
+            #pragma unroll
+            for (int u = 0; u < U; ++u) v[u] = load(e + u * a.R * a.P);
+        }
     }
-    for (; s < send; s += a.R, e += step) use(load(e), e, V);
-    if (s < t.s1 && e < E) use(part(e, (int)(E - e)), e, (int)(E - e));
+};
+
+// every vector of the thread, U in flight; the (at most one) vector that the sample's end cuts comes with its count
+template <int V, int U, typename Regs, typename Load, typename Part, typename Use>
+__device__ __forceinline__ void ga_walk(const GaArgs& a, const GaWhere& q, const GaThread& t, int E, GaFirst<V, U, Regs>* first, Load load, Part part, Use use) {
+    if (!t.on) return;
+    const int block = U * a.R, K = a.K[q.l], step = a.R * a.P;
+    int s = q.k * block + t.r;
+    unsigned e = (unsigned)s * a.P + t.v * V;   // (wraps only behind the last super-row, where it is not used)
+    if (first && first->have) {
+        #pragma unroll
+        for (int u = 0; u < U; ++u) use(first->v[u], e + u * step, V);
+        s += K * block; e += (unsigned)(K * U) * step;
+    }
+    for (; s + (U - 1) * a.R < t.send; s += K * block, e += (unsigned)(K * U) * step) {
+        Regs v[U];
+        #pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = load(e + u * step);
+        #pragma unroll
+        for (int u = 0; u < U; ++u) use(v[u], e + u * step, V);
+    }
+    if (s > t.send) return;
+    Regs v[U];   // the thread's last block, cut by the sample's end
+    #pragma unroll
+    for (int u = 0; u < U; ++u) if (s + u * a.R < t.send) v[u] = load(e + u * step);
+    #pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (s + u * a.R < t.send) use(v[u], e + u * step, V);
+        else if (s + u * a.R == t.send && e + u * step < (unsigned)E) use(part(e + u * step, E - e - u * step), e + u * step, E - e - u * step);
+    }
+}
+
+// the channels of the thread's V lanes and their groups, f(lane, channel, group) (one division for all of them)
+template <int V, typename F>
+__device__ __forceinline__ void ga_lanes(const GaArgs& a, const GaThread& t, F f) {
+    int c = t.on ? t.v * V % a.C : 0, g = c / a.cg, m = c - g * a.cg;
+    #pragma unroll
+    for (int i = 0; i < V; ++i) {
+        f(i, c, g);
+        ++c; ++m;
+        if (m == a.cg) { m = 0; ++g; }
+        if (c == a.C) { c = 0; g = 0; }
+    }
 }
 
 template <typename T> struct GaX { lgd_u32x4 x; };
@@ -145,7 +186,7 @@ template <typename T> __device__ __forceinline__ void ga_store_n(T* p, const lgd
 // sh[position][2] for the positions of this column block.  sh holds kGaThreads * V pairs.
 template <int V, typename A>
 __device__ __forceinline__ void ga_block_positions(const GaArgs& a, const GaThread& t, A (&s0)[V], A (&s1)[V], A* sh) {
-    const int r = threadIdx.x / a.cols, col = threadIdx.x % a.cols;
+    const int r = t.r, col = threadIdx.x - r * a.cols;
     int half = 1;
     while (half < a.R) half <<= 1;
     for (half >>= 1; half >= 1; half >>= 1) {
@@ -170,60 +211,140 @@ __device__ __forceinline__ void ga_block_positions(const GaArgs& a, const GaThre
     __syncthreads();
 }
 
-template <typename T>
+// sums over the n terms of each of ng groups: value(g, i, k) of term i, k in {0, 1}; put(2 g + k, sum).  Few groups are split over the workgroup (a
+// thread walking a whole group alone took 12 us at 512 channels), the parts meet in a tree.  Barriers inside
+template <typename Value, typename Put>
+__device__ __forceinline__ void ga_block_groups(int ng, int n, Value value, Put put) {
+    __shared__ double tmp[kGaThreads];
+    const int outs = 2 * ng;
+    if (outs > kGaThreads / 2) {
+        for (int j = threadIdx.x; j < outs; j += kGaThreads) {
+            double s = 0.0;
+            for (int i = 0; i < n; ++i) s += value(j >> 1, i, j & 1);
+            put(j, s);
+        }
+        return;
+    }
+    int slices = 1;
+    while (2 * slices * outs <= kGaThreads) slices <<= 1;
+    const int sl = threadIdx.x / outs, j = threadIdx.x - sl * outs;
+    double s = 0.0;
+    if (sl < slices) for (int i = sl; i < n; i += slices) s += value(j >> 1, i, j & 1);
+    for (slices >>= 1; slices >= 1; slices >>= 1) {
+        if (sl >= slices && sl < 2 * slices) tmp[threadIdx.x - slices * outs] = s;
+        __syncthreads();
+        if (sl < slices) s += tmp[threadIdx.x];
+        __syncthreads();
+    }
+    if (sl == 0) put(j, s);
+}
+
+template <typename T, bool UG>
 __global__ __launch_bounds__(kGaThreads) void ga_stats_kernel(GaArgs a) {
-    constexpr int V = Vec16<T>::V;
-    __shared__ double sh[kGaThreads * V * 2];
+    constexpr int V = Vec16<T>::V, S = UG ? 1 : V;
+    __shared__ double sh[kGaThreads * S * 2];
     const GaWhere q = ga_locate(a, blockIdx.x);
-    const GaThread t = ga_thread<V>(a, q);
     const int E = a.E[q.l];
+    const GaThread t = ga_thread<V>(a, E);
     const T* __restrict__ px = static_cast<const T*>(a.x[q.l]) + (size_t)q.b * E;
-    double s0[V], s1[V];
+    double s0[S], s1[S];
     #pragma unroll
-    for (int i = 0; i < V; ++i) s0[i] = s1[i] = 0.0;
-    ga_walk<V, 4, GaX<T>>(a, t, E, [&](long e) { return GaX<T>{ga_load(px + e)}; }, [&](long e, int n) { return GaX<T>{ga_load_part(px + e, n)}; },
-        [&](const GaX<T>& v, long, int) {
+    for (int i = 0; i < S; ++i) s0[i] = s1[i] = 0.0;
+    ga_walk<V, GA_U, GaX<T>>(a, q, t, E, (GaFirst<V, GA_U, GaX<T>>*)nullptr, [&](unsigned e) { return GaX<T>{ga_load(px + e)}; },
+        [&](unsigned e, int n) { return GaX<T>{ga_load_part(px + e, n)}; },
+        [&](const GaX<T>& v, unsigned, int) {
             float f[V];
             Vec16<T>::unpack(v.x, f);
             #pragma unroll
-            for (int i = 0; i < V; ++i) { const double d = f[i]; s0[i] += d; s1[i] = fma(d, d, s1[i]); }
+            for (int i = 0; i < V; ++i) { const double d = f[i]; s0[UG ? 0 : i] += d; s1[UG ? 0 : i] = fma(d, d, s1[UG ? 0 : i]); }
         });
-    ga_block_positions<V, double>(a, t, s0, s1, sh);
     double* part = a.partd + (size_t)blockIdx.x * a.W * 2;
-    if (a.nCB == 1) {   // positions -> groups
-        const int wraps = a.P / a.C;
-        for (int j = threadIdx.x; j < 2 * a.G; j += kGaThreads) {
-            const int g = j >> 1, k = j & 1;
-            double s = 0.0;
-            for (int w = 0; w < wraps; ++w)
-                for (int c = 0; c < a.cg; ++c) s += sh[2 * (w * a.C + g * a.cg + c) + k];
-            part[j] = s;
-        }
+    if constexpr (UG) {   // (whole column blocks) a thread's vectors lie in one group: its pair is all that the others need of it
+        sh[2 * threadIdx.x] = s0[0]; sh[2 * threadIdx.x + 1] = s1[0];
+        __syncthreads();
+        const GaBlock blk = ga_block<V>(a);
+        const int per = a.cg / V;
+        ga_block_groups(blk.ng, a.R * per, [&](int g, int i, int k) {
+            const int r = i / per;
+            return sh[2 * (r * a.cols + g * per + i - r * per) + k];
+        }, [&](int j, double s) { part[2 * blk.g0 + j] = s; });
     } else {
-        const int p0 = blockIdx.y * a.cols * V, np = min(a.cols * V, a.P - p0);
-        for (int j = threadIdx.x; j < 2 * np; j += kGaThreads) part[2 * (size_t)p0 + j] = sh[j];
+        ga_block_positions<V, double>(a, t, s0, s1, sh);
+        if (a.whole) {   // positions -> groups
+            const int wraps = a.nCB == 1 ? a.P / a.C : 1;
+            const GaBlock blk = ga_block<V>(a);
+            ga_block_groups(blk.ng, a.cg, [&](int g, int i, int k) {
+                const int c = g * a.cg + i;
+                double s = sh[2 * c + k];
+                for (int w = 1; w < wraps; ++w) s += sh[2 * (w * a.C + c) + k];
+                return s;
+            }, [&](int j, double s) { part[2 * blk.g0 + j] = s; });
+        } else {
+            const int p0 = blockIdx.y * a.cols * V, np = min(a.cols * V, a.P - p0);
+            for (int j = threadIdx.x; j < 2 * np; j += kGaThreads) part[2 * (size_t)p0 + j] = sh[j];
+        }
     }
 }
 
-// one wave per (map, sample, group): mean and 1 / sqrt(var + eps) from the chunks' records
-__global__ __launch_bounds__(64) void ga_finalize_kernel(GaArgs a) {
-    const int seg = blockIdx.x, g = seg % a.G, lb = seg / a.G, l = lb / a.B, b = lb % a.B, lane = threadIdx.x;
-    const int K = a.K[l], per = a.nCB == 1 ? 1 : a.cg, wraps = a.nCB == 1 ? 1 : a.W / a.C;
+// mean and 1 / sqrt(var + eps) of a group of n values with sums s0, s1
+__device__ __forceinline__ void ga_moments(double s0, double s1, double n, double eps, double& mean, double& rstd) {
+    mean = s0 / n;
+    double var = s1 / n - mean * mean;
+    var = var < 0.0 ? 0.0 : var;   // (NaN stays)
+    rstd = 1.0 / sqrt(var + eps);
+}
+
+// one workgroup per (map, sample, group): its statistics from the chunks' records
+__global__ __launch_bounds__(kGaThreads) void ga_finalize_kernel(GaArgs a) {
+    __shared__ double sh[4][2];
+    const int seg = blockIdx.x, g = seg % a.G, lb = seg / a.G, l = lb / a.B, b = lb % a.B;
+    const int K = a.K[l], per = a.whole ? 1 : a.cg, wraps = a.whole ? 1 : a.W / a.C;
     const double* p = a.partd + (size_t)(a.wg0[l] + b * K) * a.W * 2;
     double s0 = 0.0, s1 = 0.0;
     const int n = K * per * wraps;
-    for (int i = lane; i < n; i += 64) {
+    for (int i = threadIdx.x; i < n; i += kGaThreads) {
         const int k = i / (per * wraps), j = i % (per * wraps);
         const double* v = p + 2 * ((size_t)k * a.W + (j / per) * a.C + g * per + j % per);
         s0 += v[0]; s1 += v[1];
     }
     s0 = wave_sum(s0); s1 = wave_sum(s1);
-    if (lane == 0) {
-        const double cnt = (double)a.HW[l] * a.cg, m = s0 / cnt;
-        double var = s1 / cnt - m * m;
-        var = var < 0.0 ? 0.0 : var;   // (NaN stays)
-        a.stats[2 * (size_t)seg] = m;
-        a.stats[2 * (size_t)seg + 1] = 1.0 / sqrt(var + a.eps);
+    if ((threadIdx.x & 63) == 0) { sh[threadIdx.x >> 6][0] = s0; sh[threadIdx.x >> 6][1] = s1; }
+    __syncthreads();
+    if (threadIdx.x == 0)
+        ga_moments((sh[0][0] + sh[1][0]) + (sh[2][0] + sh[3][0]), (sh[0][1] + sh[1][1]) + (sh[2][1] + sh[3][1]), (double)a.HW[l] * a.cg, a.eps,
+                   a.stats[2 * (size_t)seg], a.stats[2 * (size_t)seg + 1]);
+}
+
+// sums of the K records of G pairs of one sample, by every workgroup that needs them: put(g, s0, s1).  Threads = groups x slices of the records; the
+// slices meet in LDS, in a fixed order.  P2: pair of the records.  Barriers inside
+template <typename P2, typename Put>
+__device__ __forceinline__ void ga_records(const P2* __restrict__ p, int K, int G, const GaBlock& blk, Put put) {
+    __shared__ double tmp[kGaThreads][2];
+    int sub = 1;
+    while (sub < blk.ng && sub < kGaThreads) sub <<= 1;
+    const int slices = kGaThreads / sub, sl = threadIdx.x / sub;
+    const int gend = blk.g0 + blk.ng;
+    for (int g0 = blk.g0; g0 < gend; g0 += sub) {
+        const int g = g0 + (threadIdx.x & (sub - 1));
+        double s0 = 0.0, s1 = 0.0;
+        if (g < gend) {
+            int k = sl;
+            for (; k + 3 * slices < K; k += 4 * slices) {
+                P2 v[4];
+                #pragma unroll
+                for (int u = 0; u < 4; ++u) v[u] = p[(size_t)(k + u * slices) * G + g];
+                #pragma unroll
+                for (int u = 0; u < 4; ++u) { s0 += (double)v[u].x; s1 += (double)v[u].y; }
+            }
+            for (; k < K; k += slices) { const P2 v = p[(size_t)k * G + g]; s0 += (double)v.x; s1 += (double)v.y; }
+        }
+        if (slices > 1) {
+            tmp[threadIdx.x][0] = s0; tmp[threadIdx.x][1] = s1;
+            __syncthreads();
+            if (sl == 0) for (int i = 1; i < slices; ++i) { s0 += tmp[threadIdx.x + i * sub][0]; s1 += tmp[threadIdx.x + i * sub][1]; }
+        }
+        if (sl == 0 && g < gend) put(g, s0, s1);
+        if (slices > 1) __syncthreads();
     }
 }
 
@@ -231,20 +352,33 @@ template <typename T, int ACT>
 __global__ __launch_bounds__(kGaThreads) void ga_apply_kernel(GaArgs a) {
     constexpr int V = Vec16<T>::V;
     const GaWhere q = ga_locate(a, blockIdx.x);
-    const GaThread t = ga_thread<V>(a, q);
     const int E = a.E[q.l];
+    const GaThread t = ga_thread<V>(a, E);
     const T* __restrict__ px = static_cast<const T*>(a.x[q.l]) + (size_t)q.b * E;
     T* __restrict__ po = static_cast<T*>(a.out[q.l]) + (size_t)q.b * E;
+    GaFirst<V, GA_U, GaX<T>> first;
+    first.issue(a, q, t, [&](unsigned e) { return GaX<T>{ga_stream(px + e)}; });
     double A[V], Bc[V];
-    const double* st = a.stats + 2 * (size_t)(q.l * a.B + q.b) * a.G;
-    #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const int c = t.on ? (t.v * V + i) % a.C : 0, g = c / a.cg;
+    double* gst = a.stats + 2 * (size_t)(q.l * a.B + q.b) * a.G;
+    const double* st = gst;
+    if (a.fused) {   // the statistics from the chunks' records; the sample's first workgroup leaves them for the backward
+        __shared__ double sst[2 * kGaFusedG];
+        const double n = (double)a.HW[q.l] * a.cg;
+        ga_records(reinterpret_cast<const double2*>(a.partd) + (size_t)(a.wg0[q.l] + q.b * a.K[q.l]) * a.G, a.K[q.l], a.G, ga_block<V>(a), [&](int g, double s0, double s1) {
+            double m, r;
+            ga_moments(s0, s1, n, a.eps, m, r);
+            sst[2 * g] = m; sst[2 * g + 1] = r;
+            if (q.k == 0) { gst[2 * g] = m; gst[2 * g + 1] = r; }
+        });
+        __syncthreads();
+        st = sst;
+    }
+    ga_lanes<V>(a, t, [&](int i, int c, int g) {
         A[i] = st[2 * g + 1] * (double)ga_param(a.gamma, a.ptype, c, 1.f);
         Bc[i] = fma(-st[2 * g], A[i], (double)ga_param(a.beta, a.ptype, c, 0.f));
-    }
-    ga_walk<V, 4, GaX<T>>(a, t, E, [&](long e) { return GaX<T>{ga_load(px + e)}; }, [&](long e, int n) { return GaX<T>{ga_load_part(px + e, n)}; },
-        [&](const GaX<T>& v, long e, int n) {
+    });
+    ga_walk<V, GA_U, GaX<T>>(a, q, t, E, &first, [&](unsigned e) { return GaX<T>{ga_stream(px + e)}; }, [&](unsigned e, int n) { return GaX<T>{ga_load_part(px + e, n)}; },
+        [&](const GaX<T>& v, unsigned e, int n) {
             float f[V];
             Vec16<T>::unpack(v.x, f);
             #pragma unroll
@@ -253,67 +387,62 @@ __global__ __launch_bounds__(kGaThreads) void ga_apply_kernel(GaArgs a) {
         });
 }
 
-// g = dy act'(z) and xh of one element.  ReLU: the sign of z in fp64 (A, Bc as the forward's); SiLU: z in fp32 from xh
-template <int ACT> __device__ __forceinline__ float ga_grad(float dy, float x, float xh, double A, double Bc, float ga, float be) {
-    if (ACT == kActRelu) return fma((double)x, A, Bc) <= 0.0 ? 0.f : dy;
-    if (ACT == kActSilu) {
-        const float z = __builtin_fmaf(xh, ga, be), s = ga_sigmoid(z);
-        return dy * __builtin_fmaf(z * s, 1.f - s, s);
-    }
-    return dy;
-}
-
-// per-channel constants of the backward
-template <int ACT, int V> struct GaCoef {
-    double r[V], nmr[V];     // xh = x r - mu r
-    double A[V], Bc[V];      // ReLU only
+// constants of a thread's V lanes; UG: V divides the channels of a group, so that a vector lies in one group
+template <int V, bool UG> struct GaCoef {
+    GaGroup grp[UG ? 1 : V];
     float ga[V], be[V];
     __device__ __forceinline__ void fill(const GaArgs& a, const GaWhere& q, const GaThread& t) {
         const double* st = a.stats + 2 * (size_t)(q.l * a.B + q.b) * a.G;
-        #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int c = t.on ? (t.v * V + i) % a.C : 0, g = c / a.cg;
-            r[i] = st[2 * g + 1]; nmr[i] = -st[2 * g] * r[i];
+        ga_lanes<V>(a, t, [&](int i, int c, int g) {
+            if (!UG || i == 0) grp[UG ? 0 : i] = ga_group(st, g);
             ga[i] = ga_param(a.gamma, a.ptype, c, 1.f); be[i] = ga_param(a.beta, a.ptype, c, 0.f);
-            if (ACT == kActRelu) { A[i] = r[i] * (double)ga[i]; Bc[i] = fma(-st[2 * g], A[i], (double)be[i]); }
-        }
+        });
     }
+    __device__ __forceinline__ const GaGroup& at(int i) const { return grp[UG ? 0 : i]; }
 };
 
-template <typename T, int ACT>
+template <typename T, int ACT, bool UG>
 __global__ __launch_bounds__(kGaThreads) void ga_bwd_stats_kernel(GaArgs a) {
     constexpr int V = Vec16<T>::V;
     __shared__ float sh[kGaThreads * V * 2];
     const GaWhere q = ga_locate(a, blockIdx.x);
-    const GaThread t = ga_thread<V>(a, q);
     const int E = a.E[q.l];
+    const GaThread t = ga_thread<V>(a, E);
     const T* __restrict__ px = static_cast<const T*>(a.x[q.l]) + (size_t)q.b * E;
     const T* __restrict__ pd = static_cast<const T*>(a.dy[q.l]) + (size_t)q.b * E;
-    GaCoef<ACT, V> k;
+    GaFirst<V, GA_UB, GaXD<T>> first;
+    first.issue(a, q, t, [&](unsigned e) { return GaXD<T>{ga_load(px + e), ga_load(pd + e)}; });
+    GaCoef<V, UG> k;
     k.fill(a, q, t);
     float s0[V], s1[V];
     #pragma unroll
     for (int i = 0; i < V; ++i) s0[i] = s1[i] = 0.f;
-    ga_walk<V, 2, GaXD<T>>(a, t, E, [&](long e) { return GaXD<T>{ga_load(px + e), ga_load(pd + e)}; },
-        [&](long e, int n) { return GaXD<T>{ga_load_part(px + e, n), ga_load_part(pd + e, n)}; },
-        [&](const GaXD<T>& v, long, int) {
+    ga_walk<V, GA_UB, GaXD<T>>(a, q, t, E, &first, [&](unsigned e) { return GaXD<T>{ga_load(px + e), ga_load(pd + e)}; },
+        [&](unsigned e, int n) { return GaXD<T>{ga_load_part(px + e, n), ga_load_part(pd + e, n)}; },
+        [&](const GaXD<T>& v, unsigned, int) {
             float x[V], d[V];
             Vec16<T>::unpack(v.x, x); Vec16<T>::unpack(v.d, d);   // behind a cut vector's end dy = 0: no contribution
             #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float xh = (float)fma((double)x[i], k.r[i], k.nmr[i]);
-                const float g = ga_grad<ACT>(d[i], x[i], xh, k.A[i], k.Bc[i], k.ga[i], k.be[i]);
+                const float xh = ga_xhat(x[i], k.at(i)), g = ga_grad<ACT>(d[i], x[i], xh, k.at(i), k.ga[i], k.be[i]);
                 s0[i] += g; s1[i] = __builtin_fmaf(g, xh, s1[i]);
             }
         });
     ga_block_positions<V, float>(a, t, s0, s1, sh);
     float* part = a.partf + (size_t)blockIdx.x * a.W * 2;
-    if (a.nCB == 1) {   // positions -> channels
-        const int wraps = a.P / a.C;
-        for (int j = threadIdx.x; j < 2 * a.C; j += kGaThreads) {
-            float s = 0.f;
-            for (int w = 0; w < wraps; ++w) s += sh[2 * w * a.C + j];
-            part[j] = s;
+    if (a.whole) {   // positions -> channels, and with gamma -> groups
+        const int wraps = a.nCB == 1 ? a.P / a.C : 1;
+        const GaBlock blk = ga_block<V>(a);
+        for (int j = threadIdx.x; j < 2 * blk.nc; j += kGaThreads) {
+            float s = sh[j];
+            for (int w = 1; w < wraps; ++w) s += sh[2 * w * a.C + j];
+            part[2 * blk.c0 + j] = s;
+            sh[j] = s * ga_param(a.gamma, a.ptype, blk.c0 + (j >> 1), 1.f);   // (j is read and written by this thread only)
+        }
+        if (a.fused) {
+            float* gp = a.partg + (size_t)blockIdx.x * a.G * 2;
+            __syncthreads();
+            ga_block_groups(blk.ng, a.cg, [&](int g, int i, int k) { return (double)sh[2 * (g * a.cg + i) + k]; }, [&](int j, double s) { gp[2 * blk.g0 + j] = (float)s; });
         }
     } else {
         const int p0 = blockIdx.y * a.cols * V, np = min(a.cols * V, a.P - p0);
@@ -321,36 +450,54 @@ __global__ __launch_bounds__(kGaThreads) void ga_bwd_stats_kernel(GaArgs a) {
     }
 }
 
-// one wave per (map, sample, group): channel sums over the chunks (kept for dgamma / dbeta) and the group's two means.  Lanes = `sub` channels x
-// 64 / sub chunk slices (sub a power of two); slices meet by an xor butterfly, in a fixed order
-__global__ __launch_bounds__(64) void ga_bwd_finalize_kernel(GaArgs a) {
-    const int seg = blockIdx.x, g = seg % a.G, lb = seg / a.G, l = lb / a.B, b = lb % a.B, lane = threadIdx.x;
-    const int K = a.K[l], wraps = a.W / a.C;
-    const float* p = a.partf + (size_t)(a.wg0[l] + b * K) * a.W * 2;
+// one workgroup per (map, sample, group): channel sums over the chunks (kept for dgamma / dbeta) and the group's two means.  Threads = `sub` channels x
+// 256 / sub slices of the chunks (sub a power of two); the slices meet in a tree, in a fixed order.  (One wave per group left 33 - 47 us of load
+// latency in this kernel.)
+__global__ __launch_bounds__(256) void ga_bwd_finalize_kernel(GaArgs a) {
+    __shared__ double sh[256][2];
+    const int seg = blockIdx.x, g = seg % a.G, lb = seg / a.G, l = lb / a.B, b = lb % a.B, tid = threadIdx.x;
+    const int wraps = a.W / a.C, n = a.K[l] * wraps;
+    const float* p = a.partf + (size_t)(a.wg0[l] + b * a.K[l]) * a.W * 2;
     int sub = 1;
-    while (sub < a.cg && sub < 64) sub <<= 1;
+    while (sub < a.cg && sub < 256) sub <<= 1;
     double m1 = 0.0, m2 = 0.0;
     for (int c0 = 0; c0 < a.cg; c0 += sub) {
-        const int j = c0 + (lane & (sub - 1)), c = g * a.cg + j;
+        const int j = c0 + (tid & (sub - 1)), c = g * a.cg + j, slices = 256 / sub;
         double s0 = 0.0, s1 = 0.0;
-        if (j < a.cg)
-            for (int i = lane / sub; i < K * wraps; i += 64 / sub) {
-                const float* v = p + 2 * ((size_t)(i / wraps) * a.W + (i % wraps) * a.C + c);
-                s0 += (double)v[0]; s1 += (double)v[1];
+        if (j < a.cg) {
+            auto at = [&](int i) { return reinterpret_cast<const float2*>(p)[(wraps == 1 ? (size_t)i * a.W : (size_t)(i / wraps) * a.W + (i % wraps) * a.C) + c]; };
+            int i = tid / sub;
+            for (; i + 3 * slices < n; i += 4 * slices) {
+                float2 v[4];
+                #pragma unroll
+                for (int u = 0; u < 4; ++u) v[u] = at(i + u * slices);
+                #pragma unroll
+                for (int u = 0; u < 4; ++u) { s0 += (double)v[u].x; s1 += (double)v[u].y; }
             }
-        for (int o = sub; o < 64; o <<= 1) { s0 += __shfl_xor(s0, o); s1 += __shfl_xor(s1, o); }
-        if (j < a.cg && lane < sub) {
+            for (; i < n; i += slices) { const float2 v = at(i); s0 += (double)v.x; s1 += (double)v.y; }
+        }
+        sh[tid][0] = s0; sh[tid][1] = s1;
+        __syncthreads();
+        for (int o = 128; o >= sub; o >>= 1) {
+            if (tid < o) { sh[tid][0] += sh[tid + o][0]; sh[tid][1] += sh[tid + o][1]; }
+            __syncthreads();
+        }
+        if (tid < sub && j < a.cg) {
+            s0 = sh[tid][0]; s1 = sh[tid][1];
             a.csum[2 * ((size_t)lb * a.C + c)] = s0;
             a.csum[2 * ((size_t)lb * a.C + c) + 1] = s1;
             const double ga = (double)ga_param(a.gamma, a.ptype, c, 1.f);
             m1 = fma(ga, s0, m1); m2 = fma(ga, s1, m2);
         }
+        __syncthreads();
     }
     m1 = wave_sum(m1); m2 = wave_sum(m2);
-    if (lane == 0) {
+    if ((tid & 63) == 0) { sh[tid >> 6][0] = m1; sh[tid >> 6][1] = m2; }
+    __syncthreads();
+    if (tid == 0) {
         const double cnt = (double)a.HW[l] * a.cg;
-        a.bstats[2 * (size_t)seg] = (float)(m1 / cnt);
-        a.bstats[2 * (size_t)seg + 1] = (float)(m2 / cnt);
+        a.bstats[2 * (size_t)seg] = (float)(((sh[0][0] + sh[1][0]) + (sh[2][0] + sh[3][0])) / cnt);
+        a.bstats[2 * (size_t)seg + 1] = (float)(((sh[0][1] + sh[1][1]) + (sh[2][1] + sh[3][1])) / cnt);
     }
 }
 
@@ -371,36 +518,73 @@ __global__ __launch_bounds__(256) void ga_param_kernel(GaArgs a) {
     }
 }
 
-template <typename T, int ACT>
+// dgamma, dbeta of 16 channels: the channel sums of every chunk of every (map, sample); 16 channels x 16 slices of the records
+constexpr int kGaParamC = 16;
+__device__ __forceinline__ void ga_params(const GaArgs& a) {
+    __shared__ double sh[kGaThreads][2];
+    const int c = blockIdx.x * kGaParamC + (threadIdx.x & 15), sl = threadIdx.x >> 4, n = a.wg0[LGD_MAX_LEVELS];
+    const float2* __restrict__ p = reinterpret_cast<const float2*>(a.partf);
+    double s0 = 0.0, s1 = 0.0;
+    if (c < a.C) {
+        int i = sl;
+        for (; i + 7 * 16 < n; i += 8 * 16) {
+            float2 v[8];
+            #pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = p[(size_t)(i + u * 16) * a.C + c];
+            #pragma unroll
+            for (int u = 0; u < 8; ++u) { s0 += (double)v[u].x; s1 += (double)v[u].y; }
+        }
+        for (; i < n; i += 16) { const float2 v = p[(size_t)i * a.C + c]; s0 += (double)v.x; s1 += (double)v.y; }
+    }
+    sh[threadIdx.x][0] = s0; sh[threadIdx.x][1] = s1;
+    __syncthreads();
+    if (sl == 0 && c < a.C) {
+        for (int i = 1; i < 16; ++i) { s0 += sh[threadIdx.x + 16 * i][0]; s1 += sh[threadIdx.x + 16 * i][1]; }
+        if (a.dbeta) ga_param_store(a.dbeta, a.ptype, c, (float)s0);
+        if (a.dgamma) ga_param_store(a.dgamma, a.ptype, c, (float)s1);
+    }
+}
+__global__ __launch_bounds__(kGaThreads) void ga_params_kernel(GaArgs a) { ga_params(a); }
+
+template <typename T, int ACT, bool UG>
 __global__ __launch_bounds__(kGaThreads) void ga_bwd_apply_kernel(GaArgs a) {
     constexpr int V = Vec16<T>::V;
-    const GaWhere q = ga_locate(a, blockIdx.x);
-    const GaThread t = ga_thread<V>(a, q);
+    if ((int)blockIdx.x < a.nparam) {   // the first workgroups of a fused call: dgamma, dbeta out of all the chunks' channel sums
+        ga_params(a);
+        return;
+    }
+    const GaWhere q = ga_locate(a, blockIdx.x - a.nparam);
     const int E = a.E[q.l];
+    const GaThread t = ga_thread<V>(a, E);
     const T* __restrict__ px = static_cast<const T*>(a.x[q.l]) + (size_t)q.b * E;
     const T* __restrict__ pd = static_cast<const T*>(a.dy[q.l]) + (size_t)q.b * E;
     T* __restrict__ po = static_cast<T*>(a.out[q.l]) + (size_t)q.b * E;
-    GaCoef<ACT, V> k;
-    k.fill(a, q, t);
-    float c1[V], c2[V], c3[V];
+    GaFirst<V, GA_UB, GaXD<T>> first;
+    first.issue(a, q, t, [&](unsigned e) { return GaXD<T>{ga_stream(px + e), ga_stream(pd + e)}; });
     const float* bs = a.bstats + 2 * (size_t)(q.l * a.B + q.b) * a.G;
-    #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const int c = t.on ? (t.v * V + i) % a.C : 0, g = c / a.cg;
-        c1[i] = (float)(k.r[i] * (double)k.ga[i]);
-        c2[i] = (float)(-k.r[i] * (double)bs[2 * g + 1]);
-        c3[i] = (float)(-k.r[i] * (double)bs[2 * g]);
+    if (a.fused) {   // the two means from the chunks' records
+        __shared__ float sbs[2 * kGaFusedG];
+        const double n = (double)a.HW[q.l] * a.cg;
+        ga_records(reinterpret_cast<const float2*>(a.partg) + (size_t)(a.wg0[q.l] + q.b * a.K[q.l]) * a.G, a.K[q.l], a.G, ga_block<V>(a),
+                   [&](int g, double s0, double s1) { sbs[2 * g] = (float)(s0 / n); sbs[2 * g + 1] = (float)(s1 / n); });
+        __syncthreads();
+        bs = sbs;
     }
-    ga_walk<V, 2, GaXD<T>>(a, t, E, [&](long e) { return GaXD<T>{ga_load(px + e), ga_load(pd + e)}; },
-        [&](long e, int n) { return GaXD<T>{ga_load_part(px + e, n), ga_load_part(pd + e, n)}; },
-        [&](const GaXD<T>& v, long e, int n) {
+    GaCoef<V, UG> k;
+    k.fill(a, q, t);
+    float c2[UG ? 1 : V], c3[UG ? 1 : V];
+    ga_lanes<V>(a, t, [&](int i, int, int g) {
+        if (!UG || i == 0) { c2[UG ? 0 : i] = -k.at(i).r * bs[2 * g + 1]; c3[UG ? 0 : i] = -k.at(i).r * bs[2 * g]; }
+    });
+    ga_walk<V, GA_UB, GaXD<T>>(a, q, t, E, &first, [&](unsigned e) { return GaXD<T>{ga_stream(px + e), ga_stream(pd + e)}; },
+        [&](unsigned e, int n) { return GaXD<T>{ga_load_part(px + e, n), ga_load_part(pd + e, n)}; },
+        [&](const GaXD<T>& v, unsigned e, int n) {
             float x[V], d[V];
             Vec16<T>::unpack(v.x, x); Vec16<T>::unpack(v.d, d);
             #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float xh = (float)fma((double)x[i], k.r[i], k.nmr[i]);
-                const float g = ga_grad<ACT>(d[i], x[i], xh, k.A[i], k.Bc[i], k.ga[i], k.be[i]);
-                d[i] = __builtin_fmaf(c1[i], g, __builtin_fmaf(c2[i], xh, c3[i]));
+                const float xh = ga_xhat(x[i], k.at(i)), g = ga_grad<ACT>(d[i], x[i], xh, k.at(i), k.ga[i], k.be[i]);
+                d[i] = __builtin_fmaf(k.at(i).r * k.ga[i], g, __builtin_fmaf(c2[UG ? 0 : i], xh, c3[UG ? 0 : i]));
             }
             ga_store_n(po + e, Vec16<T>::pack(d), n);
         });
@@ -408,7 +592,7 @@ __global__ __launch_bounds__(kGaThreads) void ga_bwd_apply_kernel(GaArgs a) {
 
 static int ga_gcd(int a, int b) { while (b) { const int t = a % b; a = b; b = t; } return a; }
 
-// the split of a call: super-rows, column blocks and chunks.  Chunks are about total / 2048 (eight workgroups of 256 threads per CU), 16 KB at least.
+// the split of a call: super-rows, column blocks and chunks
 static int ga_plan(GaArgs& a, const int32_t* hw, int L, int B, int C, int G, int dtype) {
     if (!hw || L < 1 || L > LGD_MAX_LEVELS || B < 1 || C < 1 || G < 1 || C % G || (dtype != LGD_F32 && dtype != LGD_BF16 && dtype != LGD_F16)) return LGD_EINVAL;
     const int size = dtype == LGD_F32 ? 4 : 2, V = 16 / size;
@@ -418,30 +602,48 @@ static int ga_plan(GaArgs& a, const int32_t* hw, int L, int B, int C, int G, int
     a.P = C / ga_gcd(C, V) * V; a.PV = a.P / V;
     a.nCB = (a.PV + kGaThreads - 1) / kGaThreads;
     a.cols = (a.PV + a.nCB - 1) / a.nCB;
+    a.whole = a.nCB == 1;
+    if (!a.whole && a.P == C) {   // column blocks of whole groups, where one fits
+        const int unit = a.cg / ga_gcd(a.cg, V);   // vectors of lcm(cg, V) channels
+        if (unit <= kGaThreads) {
+            a.cols = (a.cols + unit - 1) / unit * unit;
+            if (a.cols > kGaThreads) a.cols = kGaThreads / unit * unit;
+            a.nCB = (a.PV + a.cols - 1) / a.cols;
+            a.whole = 1;
+        }
+    }
     a.R = kGaThreads / a.cols;
     long long total = 0;
     for (int l = 0; l < L; ++l) {
         if (hw[2 * l] < 1 || hw[2 * l + 1] < 1) return LGD_EINVAL;
         const long long n = (long long)hw[2 * l] * hw[2 * l + 1], e = n > (1LL << 31) ? n : n * C;
-        if (e + 4LL * kGaThreads * a.P >= (1LL << 31)) return LGD_EINVAL;   // in-sample offsets are 32 bits
+        if (e + 8LL * a.R * a.P >= (1LL << 31)) return LGD_EINVAL;   // in-sample offsets are 32 bits
         a.E[l] = (int)e; a.HW[l] = (int)n;
         total += e * B * size;
     }
-    long long bytes = total / 2048;
-    if (bytes < 16384) bytes = 16384;
-    long long w = 0;
+    long long bytes = total / GA_TARGET;
+    const long long least = total / 512 < 16384 ? 16384 : total / 512 > 32768 ? 32768 : total / 512;
+    if (bytes < least) bytes = least;
+    const long long block = 16LL * 4 * kGaThreads;   // (a block of U = 4 vectors a thread)
+    const long long cap = kGaFusedRecords / G;
+    long long w = 0, wf = 0;
     for (int l = 0; l < L; ++l) {
-        const int NS = (a.E[l] + a.P - 1) / a.P;
-        long long spc = (bytes + (long long)a.P * size - 1) / ((long long)a.P * size);
-        spc = (spc + a.R - 1) / a.R * a.R;
-        a.spc[l] = (int)(spc < NS ? spc : NS);
-        a.K[l] = (NS + a.spc[l] - 1) / a.spc[l];
+        const long long sample = (long long)a.E[l] * size, want = (sample + bytes - 1) / bytes, most = (sample + block - 1) / block;
+        const long long k = want < most ? want : most;
+        a.K[l] = (int)k;
+        w += B * k;
+        wf += B * (k < cap ? k : cap);
+    }
+    if (w > 0x3fffffffLL || (long long)L * B * G > 0x7fffffffLL) return LGD_EINVAL;
+    // one kernel less where the records are few enough without leaving the chip short of workgroups
+    a.fused = a.whole && G <= kGaFusedG && cap >= 1 && (wf == w || wf >= 512);
+    w = 0;
+    for (int l = 0; l < L; ++l) {
+        if (a.fused && a.K[l] > cap) a.K[l] = (int)cap;
         a.wg0[l] = (int)w;
         w += (long long)B * a.K[l];
-        if (w > 0x7fffffffLL) return LGD_EINVAL;
     }
     for (int l = L; l <= LGD_MAX_LEVELS; ++l) a.wg0[l] = (int)w;
-    if ((long long)L * B * G > 0x7fffffffLL) return LGD_EINVAL;
     return LGD_OK;
 }
 
@@ -451,29 +653,40 @@ static size_t ga_chunks(const GaArgs& a) { return (size_t)a.wg0[LGD_MAX_LEVELS];
 template <typename T>
 static int ga_fwd(GaArgs& a, int act, hipStream_t s) {
     const dim3 grid((unsigned)ga_chunks(a), (unsigned)a.nCB);
-    LGD_LAUNCH("gn_act_stats_kernel", ga_stats_kernel<T>, grid, dim3(kGaThreads), 0, s, a);
-    LGD_LAUNCH("gn_act_finalize_kernel", ga_finalize_kernel, dim3((unsigned)(a.L * a.B * a.G)), dim3(64), 0, s, a);
+    if (a.whole && a.cg % Vec16<T>::V == 0) LGD_LAUNCH("gn_act_stats_kernel", (ga_stats_kernel<T, true>), grid, dim3(kGaThreads), 0, s, a);
+    else LGD_LAUNCH("gn_act_stats_kernel", (ga_stats_kernel<T, false>), grid, dim3(kGaThreads), 0, s, a);
+    if (!a.fused) LGD_LAUNCH("gn_act_finalize_kernel", ga_finalize_kernel, dim3((unsigned)(a.L * a.B * a.G)), dim3(kGaThreads), 0, s, a);
     if (act == kActNone) LGD_LAUNCH("gn_act_apply_kernel", (ga_apply_kernel<T, kActNone>), grid, dim3(kGaThreads), 0, s, a);
     else if (act == kActRelu) LGD_LAUNCH("gn_act_apply_kernel", (ga_apply_kernel<T, kActRelu>), grid, dim3(kGaThreads), 0, s, a);
     else LGD_LAUNCH("gn_act_apply_kernel", (ga_apply_kernel<T, kActSilu>), grid, dim3(kGaThreads), 0, s, a);
     return check_launch();
 }
 
-template <typename T, int ACT>
+template <typename T, int ACT, bool UG>
 static int ga_bwd(GaArgs& a, hipStream_t s) {
     const dim3 grid((unsigned)ga_chunks(a), (unsigned)a.nCB);
-    LGD_LAUNCH("gn_act_bwd_stats_kernel", (ga_bwd_stats_kernel<T, ACT>), grid, dim3(kGaThreads), 0, s, a);
-    LGD_LAUNCH("gn_act_bwd_finalize_kernel", ga_bwd_finalize_kernel, dim3((unsigned)(a.L * a.B * a.G)), dim3(64), 0, s, a);
-    if (a.dgamma || a.dbeta) LGD_LAUNCH("gn_act_bwd_param_kernel", ga_param_kernel, dim3((unsigned)((a.C + 63) / 64)), dim3(256), 0, s, a);
-    if (a.out[0]) LGD_LAUNCH("gn_act_bwd_apply_kernel", (ga_bwd_apply_kernel<T, ACT>), grid, dim3(kGaThreads), 0, s, a);
+    LGD_LAUNCH("gn_act_bwd_stats_kernel", (ga_bwd_stats_kernel<T, ACT, UG>), grid, dim3(kGaThreads), 0, s, a);
+    const bool params = a.dgamma || a.dbeta;
+    if (a.fused) {
+        const unsigned np = params ? (unsigned)((a.C + kGaParamC - 1) / kGaParamC) : 0u;
+        a.nparam = (int)np;
+        if (a.out[0]) LGD_LAUNCH("gn_act_bwd_apply_kernel", (ga_bwd_apply_kernel<T, ACT, UG>), dim3(grid.x + np), dim3(kGaThreads), 0, s, a);
+        else if (params) LGD_LAUNCH("gn_act_bwd_param_kernel", ga_params_kernel, dim3(np), dim3(kGaThreads), 0, s, a);
+        return check_launch();
+    }
+    LGD_LAUNCH("gn_act_bwd_finalize_kernel", ga_bwd_finalize_kernel, dim3((unsigned)(a.L * a.B * a.G)), dim3(256), 0, s, a);
+    if (params) LGD_LAUNCH("gn_act_bwd_param_kernel", ga_param_kernel, dim3((unsigned)((a.C + 63) / 64)), dim3(256), 0, s, a);
+    if (a.out[0]) LGD_LAUNCH("gn_act_bwd_apply_kernel", (ga_bwd_apply_kernel<T, ACT, UG>), grid, dim3(kGaThreads), 0, s, a);
     return check_launch();
 }
-template <typename T>
+template <typename T, bool UG>
 static int ga_bwd_act(GaArgs& a, int act, hipStream_t s) {
-    if (act == kActNone) return ga_bwd<T, kActNone>(a, s);
-    if (act == kActRelu) return ga_bwd<T, kActRelu>(a, s);
-    return ga_bwd<T, kActSilu>(a, s);
+    if (act == kActNone) return ga_bwd<T, kActNone, UG>(a, s);
+    if (act == kActRelu) return ga_bwd<T, kActRelu, UG>(a, s);
+    return ga_bwd<T, kActSilu, UG>(a, s);
 }
+template <typename T>
+static int ga_bwd_ug(GaArgs& a, int act, hipStream_t s) { return a.cg % Vec16<T>::V ? ga_bwd_act<T, false>(a, act, s) : ga_bwd_act<T, true>(a, act, s); }
 
 }  // namespace lgd
 
@@ -483,9 +696,9 @@ size_t lgd_gn_act_ws_bytes(const int32_t* level_hw_host, int L, int B, int C, in
     lgd::GaArgs a;
     if (lgd::ga_plan(a, level_hw_host, L, B, C, G, dtype) != LGD_OK) return 0;
     const size_t chunks = lgd::ga_chunks(a);
-    if (!backward) return lgd::ga_round(chunks * (size_t)(a.nCB == 1 ? G : a.P) * 2 * sizeof(double));
-    return lgd::ga_round(chunks * (size_t)(a.nCB == 1 ? C : a.P) * 2 * sizeof(float)) + lgd::ga_round((size_t)L * B * C * 2 * sizeof(double)) +
-           lgd::ga_round((size_t)L * B * G * 2 * sizeof(float));
+    if (!backward) return lgd::ga_round(chunks * (size_t)(a.whole ? G : a.P) * 2 * sizeof(double));
+    return lgd::ga_round(chunks * (size_t)(a.whole ? C : a.P) * 2 * sizeof(float)) + lgd::ga_round((size_t)L * B * C * 2 * sizeof(double)) +
+           lgd::ga_round((size_t)L * B * G * 2 * sizeof(float)) + (a.fused ? lgd::ga_round(chunks * (size_t)G * 2 * sizeof(float)) : 0);
 }
 
 int lgd_gn_act_fwd(const void* const* x_host, const int32_t* level_hw_host, int L, int B, int C, int G, int dtype, const void* gamma,
@@ -499,9 +712,13 @@ int lgd_gn_act_fwd(const void* const* x_host, const int32_t* level_hw_host, int 
         a.x[l] = x_host[l]; a.out[l] = y_host[l];
     }
     a.gamma = gamma; a.beta = beta; a.ptype = param_dtype; a.eps = eps;
-    a.W = a.nCB == 1 ? G : a.P;
+    a.W = a.whole ? G : a.P;
     a.partd = static_cast<double*>(ws); a.stats = stats;
     hipStream_t s = (hipStream_t)stream;
+    if (GA_SLAB) {
+        lgd::GaCall c = {x_host, nullptr, y_host, level_hw_host, L, B, C, G, dtype, act, param_dtype, eps, gamma, beta, stats, nullptr, nullptr, nullptr};
+        if (lgd::ga_slab_fwd(c, s)) return lgd::check_launch();
+    }
     if (dtype == LGD_F32) return lgd::ga_fwd<float>(a, act, s);
     if (dtype == LGD_BF16) return lgd::ga_fwd<__bf16>(a, act, s);
     return lgd::ga_fwd<_Float16>(a, act, s);
@@ -519,18 +736,28 @@ int lgd_gn_act_bwd(const void* const* x_host, const void* const* dy_host, const 
         a.x[l] = x_host[l]; a.dy[l] = dy_host[l]; a.out[l] = dx_host ? dx_host[l] : nullptr;
     }
     a.gamma = gamma; a.beta = beta; a.ptype = param_dtype; a.stats = const_cast<double*>(stats);
-    a.W = a.nCB == 1 ? C : a.P;
+    a.W = a.whole ? C : a.P;
     char* w = static_cast<char*>(ws);
     a.partf = reinterpret_cast<float*>(w);
     w += lgd::ga_round(lgd::ga_chunks(a) * (size_t)a.W * 2 * sizeof(float));
     a.csum = reinterpret_cast<double*>(w);
     w += lgd::ga_round((size_t)L * B * C * 2 * sizeof(double));
     a.bstats = reinterpret_cast<float*>(w);
+    w += lgd::ga_round((size_t)L * B * G * 2 * sizeof(float));
+    a.partg = reinterpret_cast<float*>(w);
     a.dgamma = dgamma; a.dbeta = dbeta;
     hipStream_t s = (hipStream_t)stream;
-    if (dtype == LGD_F32) return lgd::ga_bwd_act<float>(a, act, s);
-    if (dtype == LGD_BF16) return lgd::ga_bwd_act<__bf16>(a, act, s);
-    return lgd::ga_bwd_act<_Float16>(a, act, s);
+    if (GA_SLAB) {
+        lgd::GaCall c = {x_host, dy_host, dx_host, level_hw_host, L, B, C, G, dtype, act, param_dtype, 0.0, gamma, beta, a.stats, a.csum, dgamma, dbeta};
+        if (lgd::ga_slab_bwd(c, s)) {
+            if (L * B > 1 && (dgamma || dbeta))
+                LGD_LAUNCH("gn_act_bwd_param_kernel", lgd::ga_param_kernel, dim3((unsigned)((C + 63) / 64)), dim3(256), 0, s, a);
+            return lgd::check_launch();
+        }
+    }
+    if (dtype == LGD_F32) return lgd::ga_bwd_ug<float>(a, act, s);
+    if (dtype == LGD_BF16) return lgd::ga_bwd_ug<__bf16>(a, act, s);
+    return lgd::ga_bwd_ug<_Float16>(a, act, s);
 }
 
 }  // extern "C"
