@@ -59,7 +59,7 @@ template <int ACT> __device__ __forceinline__ float ga_grad(float dy, float x, f
     return dy * __builtin_fmaf(z * s, 1.f - s, s);
 }
 
-// a call as the one-pass kernels take it; LGD_EINVAL-free: the caller has checked it.  gn_slab.hip returns false where the call is not its own
+// a call as the one-pass kernels take it (checked by the caller); they return false where the call is not theirs
 struct GaCall {
     const void* const* x;
     const void* const* dy;
@@ -74,6 +74,7 @@ struct GaCall {
     void* dgamma;
     void* dbeta;
 };
+bool ga_slab_takes(const int32_t* hw, int L, int B, int C, int G, int dtype);
 bool ga_slab_fwd(const GaCall& c, hipStream_t s);
 bool ga_slab_bwd(const GaCall& c, hipStream_t s);
 

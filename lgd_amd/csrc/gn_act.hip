@@ -17,14 +17,8 @@
 
 namespace lgd {
 
-#ifndef GA_SLAB
-#define GA_SLAB 1
-#endif
-#ifndef GA_TARGET
-#define GA_TARGET 1024
-#define GA_U 4
-#define GA_UB 2
-#endif
+constexpr int kGaWorkgroups = 1024;    // of the streaming kernels, about: 4 per CU (768 and 2048: up to 10 and 40 % slower)
+constexpr int kGaU = 4, kGaUB = 2;     // vectors (of x; of x and dy each) of a thread in flight
 constexpr int kGaThreads = 256;
 constexpr int kGaFusedG = 512;         // groups of a fused call at most (its statistics lie in LDS) ...
 constexpr int kGaFusedRecords = 4096;  // ... and records x groups of a sample (64 KB that every workgroup of the apply kernel reads from the L2)
@@ -250,7 +244,7 @@ __global__ __launch_bounds__(kGaThreads) void ga_stats_kernel(GaArgs a) {
     double s0[S], s1[S];
     #pragma unroll
     for (int i = 0; i < S; ++i) s0[i] = s1[i] = 0.0;
-    ga_walk<V, GA_U, GaX<T>>(a, q, t, E, (GaFirst<V, GA_U, GaX<T>>*)nullptr, [&](unsigned e) { return GaX<T>{ga_load(px + e)}; },
+    ga_walk<V, kGaU, GaX<T>>(a, q, t, E, (GaFirst<V, kGaU, GaX<T>>*)nullptr, [&](unsigned e) { return GaX<T>{ga_load(px + e)}; },
         [&](unsigned e, int n) { return GaX<T>{ga_load_part(px + e, n)}; },
         [&](const GaX<T>& v, unsigned, int) {
             float f[V];
@@ -356,7 +350,7 @@ __global__ __launch_bounds__(kGaThreads) void ga_apply_kernel(GaArgs a) {
     const GaThread t = ga_thread<V>(a, E);
     const T* __restrict__ px = static_cast<const T*>(a.x[q.l]) + (size_t)q.b * E;
     T* __restrict__ po = static_cast<T*>(a.out[q.l]) + (size_t)q.b * E;
-    GaFirst<V, GA_U, GaX<T>> first;
+    GaFirst<V, kGaU, GaX<T>> first;
     first.issue(a, q, t, [&](unsigned e) { return GaX<T>{ga_stream(px + e)}; });
     double A[V], Bc[V];
     double* gst = a.stats + 2 * (size_t)(q.l * a.B + q.b) * a.G;
@@ -377,7 +371,7 @@ __global__ __launch_bounds__(kGaThreads) void ga_apply_kernel(GaArgs a) {
         A[i] = st[2 * g + 1] * (double)ga_param(a.gamma, a.ptype, c, 1.f);
         Bc[i] = fma(-st[2 * g], A[i], (double)ga_param(a.beta, a.ptype, c, 0.f));
     });
-    ga_walk<V, GA_U, GaX<T>>(a, q, t, E, &first, [&](unsigned e) { return GaX<T>{ga_stream(px + e)}; }, [&](unsigned e, int n) { return GaX<T>{ga_load_part(px + e, n)}; },
+    ga_walk<V, kGaU, GaX<T>>(a, q, t, E, &first, [&](unsigned e) { return GaX<T>{ga_stream(px + e)}; }, [&](unsigned e, int n) { return GaX<T>{ga_load_part(px + e, n)}; },
         [&](const GaX<T>& v, unsigned e, int n) {
             float f[V];
             Vec16<T>::unpack(v.x, f);
@@ -410,14 +404,14 @@ __global__ __launch_bounds__(kGaThreads) void ga_bwd_stats_kernel(GaArgs a) {
     const GaThread t = ga_thread<V>(a, E);
     const T* __restrict__ px = static_cast<const T*>(a.x[q.l]) + (size_t)q.b * E;
     const T* __restrict__ pd = static_cast<const T*>(a.dy[q.l]) + (size_t)q.b * E;
-    GaFirst<V, GA_UB, GaXD<T>> first;
+    GaFirst<V, kGaUB, GaXD<T>> first;
     first.issue(a, q, t, [&](unsigned e) { return GaXD<T>{ga_load(px + e), ga_load(pd + e)}; });
     GaCoef<V, UG> k;
     k.fill(a, q, t);
     float s0[V], s1[V];
     #pragma unroll
     for (int i = 0; i < V; ++i) s0[i] = s1[i] = 0.f;
-    ga_walk<V, GA_UB, GaXD<T>>(a, q, t, E, &first, [&](unsigned e) { return GaXD<T>{ga_load(px + e), ga_load(pd + e)}; },
+    ga_walk<V, kGaUB, GaXD<T>>(a, q, t, E, &first, [&](unsigned e) { return GaXD<T>{ga_load(px + e), ga_load(pd + e)}; },
         [&](unsigned e, int n) { return GaXD<T>{ga_load_part(px + e, n), ga_load_part(pd + e, n)}; },
         [&](const GaXD<T>& v, unsigned, int) {
             float x[V], d[V];
@@ -559,7 +553,7 @@ __global__ __launch_bounds__(kGaThreads) void ga_bwd_apply_kernel(GaArgs a) {
     const T* __restrict__ px = static_cast<const T*>(a.x[q.l]) + (size_t)q.b * E;
     const T* __restrict__ pd = static_cast<const T*>(a.dy[q.l]) + (size_t)q.b * E;
     T* __restrict__ po = static_cast<T*>(a.out[q.l]) + (size_t)q.b * E;
-    GaFirst<V, GA_UB, GaXD<T>> first;
+    GaFirst<V, kGaUB, GaXD<T>> first;
     first.issue(a, q, t, [&](unsigned e) { return GaXD<T>{ga_stream(px + e), ga_stream(pd + e)}; });
     const float* bs = a.bstats + 2 * (size_t)(q.l * a.B + q.b) * a.G;
     if (a.fused) {   // the two means from the chunks' records
@@ -576,7 +570,7 @@ __global__ __launch_bounds__(kGaThreads) void ga_bwd_apply_kernel(GaArgs a) {
     ga_lanes<V>(a, t, [&](int i, int, int g) {
         if (!UG || i == 0) { c2[UG ? 0 : i] = -k.at(i).r * bs[2 * g + 1]; c3[UG ? 0 : i] = -k.at(i).r * bs[2 * g]; }
     });
-    ga_walk<V, GA_UB, GaXD<T>>(a, q, t, E, &first, [&](unsigned e) { return GaXD<T>{ga_stream(px + e), ga_stream(pd + e)}; },
+    ga_walk<V, kGaUB, GaXD<T>>(a, q, t, E, &first, [&](unsigned e) { return GaXD<T>{ga_stream(px + e), ga_stream(pd + e)}; },
         [&](unsigned e, int n) { return GaXD<T>{ga_load_part(px + e, n), ga_load_part(pd + e, n)}; },
         [&](const GaXD<T>& v, unsigned e, int n) {
             float x[V], d[V];
@@ -621,7 +615,7 @@ static int ga_plan(GaArgs& a, const int32_t* hw, int L, int B, int C, int G, int
         a.E[l] = (int)e; a.HW[l] = (int)n;
         total += e * B * size;
     }
-    long long bytes = total / GA_TARGET;
+    long long bytes = total / kGaWorkgroups;
     const long long least = total / 512 < 16384 ? 16384 : total / 512 > 32768 ? 32768 : total / 512;
     if (bytes < least) bytes = least;
     const long long block = 16LL * 4 * kGaThreads;   // (a block of U = 4 vectors a thread)
@@ -694,8 +688,9 @@ extern "C" {
 
 size_t lgd_gn_act_ws_bytes(const int32_t* level_hw_host, int L, int B, int C, int G, int dtype, int backward) {
     lgd::GaArgs a;
-    if (lgd::ga_plan(a, level_hw_host, L, B, C, G, dtype) != LGD_OK) return 0;
+    if (lgd::ga_plan(a, level_hw_host, L, B, C, G, dtype) != LGD_OK) return (size_t)-1;
     const size_t chunks = lgd::ga_chunks(a);
+    if (lgd::ga_slab_takes(level_hw_host, L, B, C, G, dtype)) return backward && L * B > 1 ? lgd::ga_round((size_t)L * B * C * 2 * sizeof(double)) : 0;
     if (!backward) return lgd::ga_round(chunks * (size_t)(a.whole ? G : a.P) * 2 * sizeof(double));
     return lgd::ga_round(chunks * (size_t)(a.whole ? C : a.P) * 2 * sizeof(float)) + lgd::ga_round((size_t)L * B * C * 2 * sizeof(double)) +
            lgd::ga_round((size_t)L * B * G * 2 * sizeof(float)) + (a.fused ? lgd::ga_round(chunks * (size_t)G * 2 * sizeof(float)) : 0);
@@ -704,7 +699,7 @@ size_t lgd_gn_act_ws_bytes(const int32_t* level_hw_host, int L, int B, int C, in
 int lgd_gn_act_fwd(const void* const* x_host, const int32_t* level_hw_host, int L, int B, int C, int G, int dtype, const void* gamma,
                    const void* beta, int param_dtype, double eps, int act, void* ws, double* stats, void* const* y_host, void* stream) {
     lgd::GaArgs a;
-    if (lgd::ga_plan(a, level_hw_host, L, B, C, G, dtype) != LGD_OK || !x_host || !y_host || !ws || !stats || act < 0 || act > 2 ||
+    if (lgd::ga_plan(a, level_hw_host, L, B, C, G, dtype) != LGD_OK || !x_host || !y_host || !stats || act < 0 || act > 2 ||
         param_dtype < 0 || param_dtype > 2 || !(eps >= 0.0))
         return LGD_EINVAL;
     for (int l = 0; l < L; ++l) {
@@ -715,10 +710,9 @@ int lgd_gn_act_fwd(const void* const* x_host, const int32_t* level_hw_host, int 
     a.W = a.whole ? G : a.P;
     a.partd = static_cast<double*>(ws); a.stats = stats;
     hipStream_t s = (hipStream_t)stream;
-    if (GA_SLAB) {
-        lgd::GaCall c = {x_host, nullptr, y_host, level_hw_host, L, B, C, G, dtype, act, param_dtype, eps, gamma, beta, stats, nullptr, nullptr, nullptr};
-        if (lgd::ga_slab_fwd(c, s)) return lgd::check_launch();
-    }
+    const lgd::GaCall c = {x_host, nullptr, y_host, level_hw_host, L, B, C, G, dtype, act, param_dtype, eps, gamma, beta, stats, nullptr, nullptr, nullptr};
+    if (lgd::ga_slab_fwd(c, s)) return lgd::check_launch();
+    if (!ws) return LGD_EINVAL;
     if (dtype == LGD_F32) return lgd::ga_fwd<float>(a, act, s);
     if (dtype == LGD_BF16) return lgd::ga_fwd<__bf16>(a, act, s);
     return lgd::ga_fwd<_Float16>(a, act, s);
@@ -728,33 +722,31 @@ int lgd_gn_act_bwd(const void* const* x_host, const void* const* dy_host, const 
                    const void* gamma, const void* beta, int param_dtype, int act, const double* stats, void* ws, void* const* dx_host,
                    void* dgamma, void* dbeta, void* stream) {
     lgd::GaArgs a;
-    if (lgd::ga_plan(a, level_hw_host, L, B, C, G, dtype) != LGD_OK || !x_host || !dy_host || !ws || !stats || act < 0 || act > 2 ||
-        param_dtype < 0 || param_dtype > 2)
+    if (lgd::ga_plan(a, level_hw_host, L, B, C, G, dtype) != LGD_OK || !x_host || !dy_host || !stats || act < 0 || act > 2 || param_dtype < 0 ||
+        param_dtype > 2)
         return LGD_EINVAL;
     for (int l = 0; l < L; ++l) {
         if (!x_host[l] || !dy_host[l] || (dx_host && !dx_host[l])) return LGD_EINVAL;
         a.x[l] = x_host[l]; a.dy[l] = dy_host[l]; a.out[l] = dx_host ? dx_host[l] : nullptr;
     }
-    a.gamma = gamma; a.beta = beta; a.ptype = param_dtype; a.stats = const_cast<double*>(stats);
-    a.W = a.whole ? C : a.P;
+    a.gamma = gamma; a.beta = beta; a.ptype = param_dtype; a.stats = const_cast<double*>(stats); a.dgamma = dgamma; a.dbeta = dbeta;
+    hipStream_t s = (hipStream_t)stream;
     char* w = static_cast<char*>(ws);
+    if (!w && !(lgd::ga_slab_takes(level_hw_host, L, B, C, G, dtype) && L * B == 1)) return LGD_EINVAL;
+    a.csum = reinterpret_cast<double*>(w);
+    const lgd::GaCall c = {x_host, dy_host, dx_host, level_hw_host, L, B, C, G, dtype, act, param_dtype, 0.0, gamma, beta, a.stats, a.csum, dgamma, dbeta};
+    if (lgd::ga_slab_bwd(c, s)) {
+        if (L * B > 1 && (dgamma || dbeta))
+            LGD_LAUNCH("gn_act_bwd_param_kernel", lgd::ga_param_kernel, dim3((unsigned)((C + 63) / 64)), dim3(256), 0, s, a);
+        return lgd::check_launch();
+    }
+    a.W = a.whole ? C : a.P;
+    w += lgd::ga_round((size_t)L * B * C * 2 * sizeof(double));
     a.partf = reinterpret_cast<float*>(w);
     w += lgd::ga_round(lgd::ga_chunks(a) * (size_t)a.W * 2 * sizeof(float));
-    a.csum = reinterpret_cast<double*>(w);
-    w += lgd::ga_round((size_t)L * B * C * 2 * sizeof(double));
     a.bstats = reinterpret_cast<float*>(w);
     w += lgd::ga_round((size_t)L * B * G * 2 * sizeof(float));
     a.partg = reinterpret_cast<float*>(w);
-    a.dgamma = dgamma; a.dbeta = dbeta;
-    hipStream_t s = (hipStream_t)stream;
-    if (GA_SLAB) {
-        lgd::GaCall c = {x_host, dy_host, dx_host, level_hw_host, L, B, C, G, dtype, act, param_dtype, 0.0, gamma, beta, a.stats, a.csum, dgamma, dbeta};
-        if (lgd::ga_slab_bwd(c, s)) {
-            if (L * B > 1 && (dgamma || dbeta))
-                LGD_LAUNCH("gn_act_bwd_param_kernel", lgd::ga_param_kernel, dim3((unsigned)((C + 63) / 64)), dim3(256), 0, s, a);
-            return lgd::check_launch();
-        }
-    }
     if (dtype == LGD_F32) return lgd::ga_bwd_ug<float>(a, act, s);
     if (dtype == LGD_BF16) return lgd::ga_bwd_ug<__bf16>(a, act, s);
     return lgd::ga_bwd_ug<_Float16>(a, act, s);

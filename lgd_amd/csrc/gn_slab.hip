@@ -27,7 +27,7 @@ struct SlabArgs {
     const void* gamma;
     const void* beta;
     double* stats;
-    double* csum;
+    double* csum;                    // for the parameter kernel; null when one (map, sample) is all there is
     void* dgamma;                    // set when one (map, sample) is all there is: written here
     void* dbeta;
 };
@@ -273,8 +273,10 @@ __device__ __forceinline__ void slab_bwd_body(const SlabArgs& a, const SlabWhere
     for (int j = t; j < Cs; j += blockDim.x) {
         const float u0 = ch[j][0], u1 = sh[j];
         ch[j][1] = u1;
-        double* o = a.csum + 2 * ((size_t)lb * a.C + cb + j);
-        o[0] = (double)u0; o[1] = (double)u1;
+        if (a.csum) {
+            double* o = a.csum + 2 * ((size_t)lb * a.C + cb + j);
+            o[0] = (double)u0; o[1] = (double)u1;
+        }
         if (a.dbeta) ga_param_store(a.dbeta, a.ptype, cb + j, u0);
         if (a.dgamma) ga_param_store(a.dgamma, a.ptype, cb + j, u1);
     }
@@ -335,6 +337,7 @@ __global__ __launch_bounds__(kSlabThreads) void slab_bwd_kernel(SlabArgs a) {
 // the split of a call: dwords of an atom, registers, threads.  false: not a call for these kernels
 struct SlabPlan { int VW, NT; bool large, multi; };
 static bool slab_plan(SlabArgs& a, SlabPlan& p, const GaCall& c) {
+    const bool shape_only = !c.x;
     const int size = c.dtype == LGD_F32 ? 4 : 2, cg = c.C / c.G;
     int most = 0;
     for (int l = 0; l < c.L; ++l) { const int n = c.hw[2 * l] * c.hw[2 * l + 1]; most = n > most ? n : most; }
@@ -380,7 +383,8 @@ static bool slab_plan(SlabArgs& a, SlabPlan& p, const GaCall& c) {
         for (int l = 0; l < LGD_MAX_LEVELS; ++l) {
             a.wg0[l] = (int)w;
             if (l >= c.L) continue;
-            a.x[l] = c.x[l]; a.dy[l] = c.dy ? c.dy[l] : nullptr; a.out[l] = c.out ? c.out[l] : nullptr;
+            if (!shape_only) a.x[l] = c.x[l];
+            a.dy[l] = c.dy ? c.dy[l] : nullptr; a.out[l] = c.out ? c.out[l] : nullptr;
             a.HW[l] = c.hw[2 * l] * c.hw[2 * l + 1];
             w += ((long long)a.cnt + 7) / 8 * 8;
             if (w > 0x3fffffffLL) return false;
@@ -420,6 +424,14 @@ template <typename T> static void slab_fwd_vw(const SlabArgs& a, const SlabPlan&
 }
 template <typename T> static void slab_bwd_vw(const SlabArgs& a, const SlabPlan& p, hipStream_t s) {
     if (p.VW == 4) slab_bwd_launch<T, 4>(a, p, s); else if (p.VW == 2) slab_bwd_launch<T, 2>(a, p, s); else slab_bwd_launch<T, 1>(a, p, s);
+}
+
+bool ga_slab_takes(const int32_t* hw, int L, int B, int C, int G, int dtype) {
+    SlabArgs a;
+    SlabPlan p;
+    GaCall c = {};
+    c.hw = hw; c.L = L; c.B = B; c.C = C; c.G = G; c.dtype = dtype;
+    return slab_plan(a, p, c);
 }
 
 bool ga_slab_fwd(const GaCall& c, hipStream_t s) {

@@ -83,7 +83,7 @@ def grad_norm(tensors, norm_type=2.0):
     with hip.device_guard(device):
         out = torch.empty((), dtype=torch.float32, device=device)
         ws = torch.empty(lib.lgd_grad_norm_ws_bytes(len(rec)), dtype=torch.uint8, device=device)
-        hip.check(lib.lgd_grad_norm(ctypes.c_void_p(rec.ctypes.data), len(rec), code, hip.ptr(ws), hip.ptr(out), hip.stream_ptr()), "lgd_grad_norm")
+        hip.check(lib.lgd_grad_norm(rec.ctypes.data, len(rec), code, ws.data_ptr(), out.data_ptr(), hip.stream_ptr()), "lgd_grad_norm")
     return out
 
 
@@ -108,8 +108,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0):
     with hip.device_guard(device):
         out = torch.empty((), dtype=torch.float32, device=device)
         ws = torch.empty(lib.lgd_grad_norm_ws_bytes(len(rec)), dtype=torch.uint8, device=device)
-        hip.check(lib.lgd_grad_clip(ctypes.c_void_p(rec.ctypes.data), len(rec), code, ctypes.c_float(max_norm), hip.ptr(ws), hip.ptr(out),
-                                    hip.stream_ptr()), "lgd_grad_clip")
+        hip.check(lib.lgd_grad_clip(rec.ctypes.data, len(rec), code, max_norm, ws.data_ptr(), out.data_ptr(), hip.stream_ptr()), "lgd_grad_clip")
         if flat is not grads:
             for g, f in zip(grads, flat):
                 if f is not g:

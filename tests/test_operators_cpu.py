@@ -94,13 +94,15 @@ def test_c_entries_refuse_bad_arguments(lib):
     fwd = lambda x=ptrs, hw=hw, L=1, B=1, C=6, G=2, dt=0, pt=0, eps=1e-5, act=0, ws=one, st=one, y=ptrs: lib.lgd_gn_act_fwd(  # noqa: E731
         x, hw, L, B, C, G, dt, None, None, pt, eps, act, ws, st, y, None)
     for bad in (dict(x=None), dict(x=none), dict(y=None), dict(y=none), dict(L=0), dict(L=17), dict(B=0), dict(C=0), dict(G=0), dict(G=4), dict(dt=3),
-                dict(dt=-1), dict(pt=3), dict(eps=-1.0), dict(eps=float("nan")), dict(act=3), dict(act=-1), dict(ws=None), dict(st=None),
+                dict(dt=-1), dict(pt=3), dict(eps=-1.0), dict(eps=float("nan")), dict(act=3), dict(act=-1), dict(hw=hip.int_array([80, 800]), ws=None), dict(st=None),
                 dict(hw=hip.int_array([0, 8])), dict(hw=None), dict(hw=big)):
         assert fwd(**bad) == -1, bad
     assert lib.lgd_gn_act_bwd(ptrs, None, hw, 1, 1, 6, 2, 0, None, None, 0, 0, one, one, ptrs, None, None, None) == -1
-    assert lib.lgd_gn_act_bwd(ptrs, ptrs, hw, 1, 1, 6, 2, 0, None, None, 0, 0, None, one, ptrs, None, None, None) == -1
+    assert lib.lgd_gn_act_bwd(ptrs, ptrs, hw, 1, 2, 6, 2, 0, None, None, 0, 0, None, one, ptrs, None, None, None) == -1   # the workspace
     assert lib.lgd_gn_act_bwd(ptrs, ptrs, hw, 1, 1, 6, 2, 0, None, None, 0, 0, one, one, none, None, None, None) == -1
-    assert lib.lgd_gn_act_ws_bytes(big, 1, 1, 6, 2, 0, 0) == 0 and lib.lgd_gn_act_ws_bytes(hw, 1, 1, 6, 2, 0, 0) > 0
+    bytes_of = lambda hw, B, back: lib.lgd_gn_act_ws_bytes(hw, 1, B, 6, 2, 0, back)  # noqa: E731
+    assert bytes_of(big, 1, 0) == bytes_of(big, 1, 1) == ops._NO_CALL and bytes_of(hip.int_array([80, 800]), 1, 0) > 0
+    assert bytes_of(hw, 2, 0) == 0 and bytes_of(hw, 1, 1) == 0 and bytes_of(hw, 2, 1) > 0   # small: no workspace but for the parameters' gradients
 
     def norm(rec, n=1, kind=0, ws=one, out=one, clip=None):
         r = (hip.GradTensor * 1)(rec)
