@@ -5,8 +5,8 @@ logic stays testable) but any kernel call raises LgdHipError when the library or
 GPU is missing -- the product path must fail loudly rather than silently compute
 elsewhere.
 """
-import contextlib
 import ctypes
+import importlib.util
 import os
 
 import torch
@@ -159,10 +159,6 @@ class GradTensor(ctypes.Structure):
     _fields_ = [("p", c_fp), ("n", ctypes.c_int64), ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
-# element types of the entry points that take more than fp32 (LGD_F32 / LGD_BF16 / LGD_F16)
-DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-
-
 class LgdHipError(RuntimeError):
     pass
 
@@ -190,6 +186,26 @@ def load():
     return lib
 
 
+_HOST_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "_lgd_host.so")
+_HOST_ENTRIES = ("lgd_gn_act_ws_bytes", "lgd_gn_act_fwd", "lgd_gn_act_bwd", "lgd_grad_norm_ws_bytes", "lgd_grad_norm", "lgd_grad_clip", "lgd_last_error")
+_host = None
+
+
+def host():
+    """the CPython extension of csrc/host.cpp (idempotent), bound to the kernel library's entry points."""
+    global _host
+    if _host is None:
+        lib = load()
+        if not os.path.exists(_HOST_PATH):
+            raise LgdHipError("host extension missing: %s -- run `python -c 'import __graft_entry__ as g; g.build()'`" % _HOST_PATH)
+        spec = importlib.util.spec_from_file_location("_lgd_host", _HOST_PATH)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.bind(LgdHipError, *[ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _HOST_ENTRIES])
+        _host = mod
+    return _host
+
+
 _HAS_GPU = None
 
 
@@ -214,14 +230,6 @@ def stream_ptr():
     """the current HIP stream of the current device as a void* (the raw getter: torch.cuda.current_stream() builds a Stream object
     and resolves the device index in Python, ~9 us per call x ~300 calls per step)."""
     return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
-
-
-_SAME_DEVICE = contextlib.nullcontext()
-
-
-def device_guard(device):
-    """context that makes `device` the current one (stream_ptr() and the launches follow it); free when it already is."""
-    return _SAME_DEVICE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def ptr(t):

@@ -342,169 +342,26 @@ def group_norm_relu(xs, groups, weight=None, bias=None, relu=True):
 
 
 _GN_ACTS = {"none": 0, "relu": 1, "silu": 2}   # LGD_ACT_*
-_NO_CALL = ctypes.c_size_t(-1).value
-
-
-def _dense_nhwc(t):
-    """t, or a copy of it, dense in channels-last order (any element alignment will do)."""
-    return t if t.is_contiguous(memory_format=torch.channels_last) else t.contiguous(memory_format=torch.channels_last)
-
-
-def _gn_act_check(xs, groups, weight, bias, act, eps):
-    x0 = xs[0]
-    dt, dev, bc = x0.dtype, x0.device, x0.shape[:2]
-    if act not in _GN_ACTS:
-        raise hip.LgdHipError("activation %r: one of %s" % (act, ", ".join(sorted(_GN_ACTS))))
-    if not eps >= 0:
-        raise hip.LgdHipError("eps must not be negative, got %r" % (eps,))
-    if len(xs) > 16:
-        raise hip.LgdHipError("at most 16 maps per call (LGD_MAX_LEVELS), got %d" % len(xs))
-    if dt not in hip.DTYPES:
-        raise hip.LgdHipError("group_norm_act takes fp32, bf16 or fp16 maps, got %s" % dt)
-    for x in xs:
-        if x.dim() != 4 or x.shape[:2] != bc:
-            raise hip.LgdHipError("maps of one call are (B,C,H_l,W_l) with the same B and C, got %s" % [tuple(v.shape) for v in xs])
-        if x.dtype != dt or x.device != dev or x.layout is not torch.strided:
-            raise hip.LgdHipError("maps of one call are strided, of one type and on one device, got %s" % [(v.layout, v.dtype, str(v.device)) for v in xs])
-    C = bc[1]
-    if groups < 1 or C < 1 or C % groups:
-        raise hip.LgdHipError("%d channels do not split into %d groups" % (C, groups))
-    for p in (weight, bias):
-        if p is not None and (p.dtype not in hip.DTYPES or p.dim() != 1 or p.shape[0] != C or p.device != dev):
-            raise hip.LgdHipError("%s must be %d fp32, bf16 or fp16 values on %s, got %s %s on %s"
-                                  % ("weight" if p is weight else "bias", C, dev, tuple(p.shape), p.dtype, p.device))
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise hip.LgdHipError("weight and bias have one type, got %s and %s" % (weight.dtype, bias.dtype))
-
-
-def _gn_act_meta(xs, weight, bias):
-    """(level_hw, L, B, C, map type, parameter type) of non-empty maps, as the C entries take them"""
-    B, C = xs[0].shape[:2]
-    hw = (ctypes.c_int32 * (2 * len(xs)))(*[v for x in xs for v in x.shape[2:]])
-    p = weight if weight is not None else bias
-    return hw, len(xs), B, C, hip.DTYPES[xs[0].dtype], hip.DTYPES[p.dtype] if p is not None else 0
-
-
-def _opt_ptr(t):
-    return t.data_ptr() if t is not None else None
-
-
-def _gn_act_fwd(xs, groups, weight, bias, act, eps, keep):
-    """-> (outputs, dense inputs, stats) of the maps; maps without elements pass through as they are.  keep: the statistics are kept for a
-    backward (in an allocation without the workspace)"""
-    lib = hip.load()
-    xs = [_dense_nhwc(x) for x in xs]
-    ys = [torch.empty_like(x) for x in xs]
-    xl, yl = xs, ys
-    if not all(x.numel() for x in xs):
-        live = [i for i, x in enumerate(xs) if x.numel()]
-        if not live:
-            return ys, xs, None
-        xl, yl = [xs[i] for i in live], [ys[i] for i in live]
-    hw, L, B, C, dt, pt = _gn_act_meta(xl, weight, bias)
-    dev = xl[0].device
-    if _TIMER_ON:
-        nb = xl[0].element_size() * sum(x.numel() for x in xl)
-        for name, times in (("gn_act_slab_kernel", 2), ("gn_act_stats_kernel", 1), ("gn_act_apply_kernel", 2)):
-            _count_bytes(name, times * nb)
-    with hip.device_guard(dev):
-        n = lib.lgd_gn_act_ws_bytes(hw, L, B, C, groups, dt, 0)
-        if n == _NO_CALL:
-            raise hip.LgdHipError("group_norm_act: maps of 2^31 elements per sample or more are not supported")
-        words = 2 * L * B * groups
-        if n == 0 or not keep:
-            stats = torch.empty(words + n // 8, dtype=torch.float64, device=dev)   # (n is a multiple of 256)
-            ws = stats.data_ptr() + 8 * words
-        else:
-            stats, buf = torch.empty(words, dtype=torch.float64, device=dev), torch.empty(n, dtype=torch.uint8, device=dev)
-            ws = buf.data_ptr()
-        hip.check(lib.lgd_gn_act_fwd(hip.ptr_array(xl), hw, L, B, C, groups, dt, _opt_ptr(weight), _opt_ptr(bias), pt, eps, _GN_ACTS[act],
-                                     ws if n else None, stats.data_ptr(), hip.ptr_array(yl), hip.stream_ptr()), "lgd_gn_act_fwd")
-    return ys, xs, stats
-
-
-class _FirstOnly(torch.autograd.Function):
-    """gradients computed under create_graph: they depend on `anchors` in a way no graph holds, so differentiating them again must raise."""
-    @staticmethod
-    def forward(ctx, n_anchors, *ts):
-        return tuple(t.view_as(t) for t in ts[n_anchors:])
-
-    @staticmethod
-    def backward(ctx, *grads):
-        raise hip.LgdHipError("group_norm_act has no second derivative")
-
-
-class _GroupNormAct(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, groups, act, eps, weight, bias, *xs):
-        weight = weight.contiguous() if weight is not None else None
-        bias = bias.contiguous() if bias is not None else None
-        ys, xs, stats = _gn_act_fwd(xs, groups, weight, bias, act, eps, True)
-        ctx.save_for_backward(stats, weight, bias, *xs)
-        ctx.meta = (groups, act)
-        return tuple(ys)
-
-    @staticmethod
-    def backward(ctx, *dys):
-        if not torch.is_grad_enabled():
-            return _GroupNormAct._backward(ctx, *dys)
-        with torch.no_grad():
-            got = _GroupNormAct._backward(ctx, *dys)
-        real = [i for i, g in enumerate(got) if g is not None]
-        anchors = [t for t in (*ctx.saved_tensors[1:], *dys) if t is not None and t.requires_grad]
-        out = list(got)
-        for i, g in zip(real, _FirstOnly.apply(len(anchors), *anchors, *[got[i] for i in real])):
-            out[i] = g
-        return tuple(out)
-
-    @staticmethod
-    def _backward(ctx, *dys):
-        lib = hip.load()
-        groups, act = ctx.meta
-        stats, weight, bias, *xs = ctx.saved_tensors
-        want_w, want_b, want_x = ctx.needs_input_grad[3], ctx.needs_input_grad[4], any(ctx.needs_input_grad[5:])
-        dw = torch.empty_like(weight) if want_w else None
-        db = torch.empty_like(bias) if want_b else None
-        dxs = [torch.empty_like(x) for x in xs] if want_x else None
-        xl, dxl = xs, dxs
-        if all(x.numel() for x in xs):
-            dl = [_dense_nhwc(d) for d in dys]
-        else:
-            live = [i for i, x in enumerate(xs) if x.numel()]
-            if not live:
-                return (None, None, None, dw.zero_() if want_w else None, db.zero_() if want_b else None, *(dxs or [None] * len(xs)))
-            xl, dl, dxl = [xs[i] for i in live], [_dense_nhwc(dys[i]) for i in live], [dxs[i] for i in live] if want_x else None
-        hw, L, B, C, dt, pt = _gn_act_meta(xl, weight, bias)
-        dev = xl[0].device
-        if _TIMER_ON:
-            nb = xl[0].element_size() * sum(x.numel() for x in xl)
-            for name, times in (("gn_act_bwd_slab_kernel", 3), ("gn_act_bwd_stats_kernel", 2), ("gn_act_bwd_apply_kernel", 3)):
-                _count_bytes(name, times * nb)
-        with hip.device_guard(dev):
-            n = lib.lgd_gn_act_ws_bytes(hw, L, B, C, groups, dt, 1)
-            ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-            hip.check(lib.lgd_gn_act_bwd(hip.ptr_array(xl), hip.ptr_array(dl), hw, L, B, C, groups, dt, _opt_ptr(weight), _opt_ptr(bias), pt,
-                                         _GN_ACTS[act], stats.data_ptr(), _opt_ptr(ws), hip.ptr_array(dxl) if want_x else None,
-                                         _opt_ptr(dw), _opt_ptr(db), hip.stream_ptr()), "lgd_gn_act_bwd")
-        return (None, None, None, dw, db, *(dxs or [None] * len(xs)))
 
 
 def group_norm_act(xs, groups, weight=None, bias=None, act="relu", eps=1e-5):
     """act(nn.GroupNorm(groups, C, eps)(x)) of a list of CHANNELS-LAST maps (B,C,H_l,W_l), fp32 / bf16 / fp16, with ONE module over all of
     them (group_norm_relu is the NCHW fp32 form): act "none", "relu" or "silu"; weight / bias (C,) fp32, bf16 or fp16, or None.  Maps that are
     not dense in torch.channels_last order are copied into it; the outputs and the input gradients are channels-last, in the maps' type,
-    rounded once (statistics and the sign under a ReLU are 64-bit).  A map without elements gives one without elements."""
+    rounded once (statistics and the sign under a ReLU are 64-bit).  A map without elements gives one without elements.  First derivatives only.
+    The checks, the allocations and the autograd node are csrc/host.cpp: on small maps they are most of what a call costs."""
+    code = _GN_ACTS.get(act)
+    if code is None:
+        raise hip.LgdHipError("activation %r: one of %s" % (act, ", ".join(sorted(_GN_ACTS))))
     xs = list(xs)
-    if not xs:
-        return []
-    groups, eps = int(groups), float(eps)
-    _gn_act_check(xs, groups, weight, bias, act, eps)
-    hip.require_gpu(*xs)
-    if torch.is_grad_enabled() and (any(x.requires_grad for x in xs) or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
-        return list(_GroupNormAct.apply(groups, act, eps, weight, bias, *xs))
-    return _gn_act_fwd(xs, groups, weight.contiguous() if weight is not None else None, bias.contiguous() if bias is not None else None,
-                       act, eps, False)[0]
+    if _TIMER_ON:
+        nb = sum(x.numel() * x.element_size() for x in xs)
+        for name, times in (("gn_act_slab_kernel", 2), ("gn_act_stats_kernel", 1), ("gn_act_apply_kernel", 2)):
+            _count_bytes(name, times * nb)
+    ys = hip.host().group_norm_act(xs, groups, code, eps, weight, bias)
+    if ys is None:
+        hip.require_gpu(*xs)
+    return ys
 
 
 class _GroupNormFold(torch.autograd.Function):

@@ -11,7 +11,6 @@ ops and two optimizers) and ~40 launches over 13 tensor transfers per element; a
 optimizer entry.  Here the host builds one table (three pointers, length, lr / wd / mu per tensor) in pinned memory and launches once.
 """
 import ctypes
-import operator
 
 import numpy as np
 import torch
@@ -22,13 +21,7 @@ _TENSOR_DT = np.dtype([("p", "<u8"), ("g", "<u8"), ("m", "<u8"), ("n", "<i8"), (
                        ("reserved", "<i4")])  # mirror of lgd_sgd_tensor (include/lgd_hip.h), 48 bytes
 assert _TENSOR_DT.itemsize == 48
 
-_GRAD_DT = np.dtype([("p", "<u8"), ("n", "<i8"), ("dtype", "<i4"), ("reserved", "<i4")])   # mirror of lgd_grad_tensor, 24 bytes
-assert _GRAD_DT.itemsize == ctypes.sizeof(hip.GradTensor) == 24
-
 _NORMS = {2.0: 0, 1.0: 1, float("inf"): 2}   # LGD_NORM_*
-
-
-_kind = operator.attrgetter("dtype", "device", "layout")
 
 
 def _norm_code(norm_type):
@@ -38,100 +31,33 @@ def _norm_code(norm_type):
     return code
 
 
-def _dense(t):
-    """whether t's elements fill one contiguous run of memory, in whatever order (channels-last filters do)"""
-    if t.is_contiguous():
-        return True
-    want = 1
-    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
-        if st != want:
-            return False
-        want *= n
-    return True
-
-
-def _grad_records(tensors):
-    """-> (records, dense tensors, device): every tensor as the kernels take it.  A tensor that is not one run of memory is replaced by a
-    contiguous copy."""
-    kinds = set(map(_kind, tensors))   # C-level passes over the list: what a call costs the host is per tensor
-    device = tensors[0].device
-    for dtype, dev, layout in kinds:
-        if layout is not torch.strided or dtype not in hip.DTYPES or dev != device:
-            raise hip.LgdHipError("gradient norms take strided fp32, bf16 or fp16 tensors on one device, got %s %s on %s (the first is on %s)"
-                                  % (layout, dtype, dev, device))
-    flat = tensors if all(map(torch.Tensor.is_contiguous, tensors)) else [t if _dense(t) else t.contiguous() for t in tensors]
-    n = len(flat)
-    rec = np.empty(n, dtype=_GRAD_DT)
-    rec["p"] = np.fromiter(map(torch.Tensor.data_ptr, flat), dtype=np.uint64, count=n)
-    rec["n"] = np.fromiter(map(torch.Tensor.numel, flat), dtype=np.int64, count=n)
-    rec["dtype"] = hip.DTYPES[tensors[0].dtype] if len(kinds) == 1 else [hip.DTYPES[t.dtype] for t in flat]
-    rec["reserved"] = 0
-    return rec, flat, device
-
-
-@torch.no_grad()
 def grad_norm(tensors, norm_type=2.0):
     """norm over every element of every tensor (fp32 / bf16 / fp16, mixed) as ONE vector -> 0-dim fp32 tensor on their device, no host sync:
     norm_type 2, 1 or inf.  Sums are 64-bit and run in a fixed order.  A NaN anywhere gives NaN.  No tensors: 0 on the CPU."""
-    code = _norm_code(norm_type)
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    if not tensors:
-        return torch.tensor(0.0)
-    rec, flat, device = _grad_records(tensors)
-    hip.require_gpu(tensors[0])
-    lib = hip.load()
-    with hip.device_guard(device):
-        out = torch.empty((), dtype=torch.float32, device=device)
-        ws = torch.empty(lib.lgd_grad_norm_ws_bytes(len(rec)), dtype=torch.uint8, device=device)
-        hip.check(lib.lgd_grad_norm(rec.ctypes.data, len(rec), code, ws.data_ptr(), out.data_ptr(), hip.stream_ptr()), "lgd_grad_norm")
-    return out
+    return _norm(hip.host().norm(tensors, False, _norm_code(norm_type), None), tensors)
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0):
     """clip the gradients of `parameters` (a tensor or an iterable; those without a gradient are skipped) IN PLACE by the norm of all of them
     taken together, torch.nn.utils.clip_grad_norm_'s arithmetic: g *= min(1, max_norm / (norm + 1e-6)).  -> the norm before clipping (0-dim
     fp32 on the device).  No host sync, two launches over all the tensors; nothing is written where nothing has to be clipped.  A norm that is
     not finite reaches the gradients as it does in torch (NaN everywhere, or 0 and NaN).  The gradients must not share memory."""
-    code = _norm_code(norm_type)
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise hip.LgdHipError("max_norm must not be negative, got %r" % max_norm)
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
-    grads = [p.grad for p in parameters if p.grad is not None]
-    if not grads:
+    return _norm(hip.host().norm(parameters, True, _norm_code(norm_type), max_norm), parameters)
+
+
+def _norm(got, tensors):
+    """csrc/host.cpp's answer: a tensor, None (there were no tensors) or False (they are not on a GPU)"""
+    if got is None:
         return torch.tensor(0.0)
-    rec, flat, device = _grad_records(grads)
-    _refuse_shared(rec, grads, flat)
-    hip.require_gpu(grads[0])
-    lib = hip.load()
-    with hip.device_guard(device):
-        out = torch.empty((), dtype=torch.float32, device=device)
-        ws = torch.empty(lib.lgd_grad_norm_ws_bytes(len(rec)), dtype=torch.uint8, device=device)
-        hip.check(lib.lgd_grad_clip(rec.ctypes.data, len(rec), code, max_norm, ws.data_ptr(), out.data_ptr(), hip.stream_ptr()), "lgd_grad_clip")
-        if flat is not grads:
-            for g, f in zip(grads, flat):
-                if f is not g:
-                    g.copy_(f)
-    torch.autograd.graph.increment_version(grads)   # written through raw pointers
-    return out
-
-
-def _refuse_shared(rec, grads, flat):
-    """in-place scaling needs every element once: a gradient listed twice, an expanded one, or views that overlap are refused"""
-    p = rec["p"].astype(np.int64)
-    e = p + rec["n"] * np.where(rec["dtype"] == 0, 4, 2)
-    live = e > p
-    if not live.all():
-        p, e = p[live], e[live]
-    order = np.argsort(p)
-    if bool((e[order][:-1] > p[order][1:]).any()):
-        raise hip.LgdHipError("two of the gradients share memory: each element can be clipped once")
-    if flat is grads:
-        return
-    strided = [g for g, f in zip(grads, flat) if f is not g]
-    if any(st == 0 and n > 1 for g in strided for st, n in zip(g.stride(), g.shape)) or len({g.data_ptr() for g in strided}) != len(strided):
-        raise hip.LgdHipError("a gradient that is expanded, or listed twice, cannot be clipped in place")
+    if got is False:
+        hip.require_gpu(*tensors)
+        raise hip.LgdHipError("gradients are not on a GPU")
+    return got
 
 
 def supported(optimizers, clip):
