@@ -110,7 +110,7 @@ class FusedClipSGD:
         self._state_ids = None     # Optimizer.load_state_dict installs a new state dict: the cached buffers are then stale
         self._grp = np.array([k * 4096 + gi for k, gi in self.owner], dtype=np.int64)
         self.chunk = None
-        self._checked_idx = None
+        self._checked_idx = self._plan = None
         rec = 48 * n + 4 * (n + 1)
         self._slot_bytes = (rec + 255) // 256 * 256
         self._pinned = None
@@ -159,46 +159,52 @@ class FusedClipSGD:
         hip.require_gpu(grads[idx[0]])
         if by_norm and torch.cuda.is_current_stream_capturing():
             raise hip.LgdHipError("the fused step uploads its table from host memory that later steps reuse: it cannot be captured into a graph")
-        if idx != self._checked_idx:   # layout checks once per set of parameters that receive gradients (autograd hands out the
-            for i in idx:              # same kind of tensor every step; the checks cost ~0.12 ms of the ~0.4 ms this call takes)
-                g = grads[i]
+        params = [self.params[i] for i in idx]
+        grads = [grads[i] for i in idx]
+        k = len(idx)
+        if idx != self._checked_idx:   # once per set of parameters that receive gradients: layout checks (autograd hands out the same kind of
+            for g in grads:            # tensor every step) and what the table's other columns follow from
                 if g.dtype != torch.float32 or not g.is_contiguous() or g.is_sparse:
                     raise hip.LgdHipError("fused SGD needs dense contiguous fp32 gradients")
+            ii = np.asarray(idx, dtype=np.int64)
+            tab, blk = np.zeros(k, dtype=_TENSOR_DT), np.zeros(k + 1, dtype=np.int32)
+            tab["n"] = self._numel[ii]
+            blk[1:] = np.cumsum((self._numel[ii] + self.chunk - 1) // self.chunk)
+            keys, which = np.unique(self._grp[ii], return_inverse=True)
+            owner = self._grp[ii] // 4096
+            if by_norm:
+                tab["reserved"] = owner
+            border = np.searchsorted(owner, np.arange(len(self.optimizers) + 1)).astype(np.int32)   # the table is ordered by optimizer
+            self._plan = (ii, tab, blk, [divmod(key, 4096) for key in keys.tolist()], which, border, blk[border])
             self._checked_idx = idx
+        elif not all(map(torch.Tensor.is_contiguous, grads)):
+            raise hip.LgdHipError("fused SGD needs dense contiguous fp32 gradients")
         self._buffers(idx)
-        ii = np.asarray(idx, dtype=np.int64)
-        k = len(idx)
-        device = grads[idx[0]].device
+        ii, tab, blk, keys, which, border, border_blk = self._plan
+        ptr_of = torch.Tensor.data_ptr
+        gp = list(map(ptr_of, grads))
+        if by_norm and len(set(gp)) < k and len({q for q, g in zip(gp, grads) if g.numel()}) < sum(g.numel() > 0 for g in grads):
+            raise hip.LgdHipError("two of the gradients share memory: each element can be clipped once")
+        tab["p"] = list(map(ptr_of, params))
+        tab["g"] = gp
+        tab["m"] = self._m_ptr[ii]
+        hy = np.array([[g["lr"], g["weight_decay"], g["momentum"]] for g in (self.optimizers[o].param_groups[j] for o, j in keys)], dtype=np.float32)[which]
+        tab["lr"], tab["wd"], tab["mu"] = hy[:, 0], hy[:, 1], hy[:, 2]
+        device = grads[0].device
         if self._pinned is None:
             self._pinned = torch.empty(self.SLOTS * self._slot_bytes, dtype=torch.uint8).pin_memory()
         s = self._slot
         self._slot = (s + 1) % self.SLOTS
         if self._events[s] is not None:
             self._events[s].synchronize()   # SLOTS steps old: long complete unless the host ran that far ahead
-        host = self._pinned[s * self._slot_bytes:(s + 1) * self._slot_bytes]
-        raw = host.numpy()
-        tab = raw[:48 * k].view(_TENSOR_DT)
-        blk = raw[48 * k:48 * k + 4 * (k + 1)].view(np.int32)
-        ptr_of = torch.Tensor.data_ptr
-        params = self.params
-        tab["p"] = np.fromiter(map(ptr_of, [params[i] for i in idx]), dtype=np.uint64, count=k)
-        tab["g"] = np.fromiter(map(ptr_of, [grads[i] for i in idx]), dtype=np.uint64, count=k)
-        tab["m"] = self._m_ptr[ii]
-        tab["n"] = self._numel[ii]
-        hyper = {}
-        for key in np.unique(self._grp[ii]).tolist():
-            g = self.optimizers[key // 4096].param_groups[key % 4096]
-            hyper[key] = (float(g["lr"]), float(g["weight_decay"]), float(g["momentum"]))
-        hy = np.array([hyper[key] for key in self._grp[ii].tolist()], dtype=np.float32)
-        tab["lr"], tab["wd"], tab["mu"] = hy[:, 0], hy[:, 1], hy[:, 2]
-        owner = self._grp[ii] // 4096
-        tab["reserved"] = owner if by_norm else 0
-        blk[0] = 0
-        blk[1:] = np.cumsum((self._numel[ii] + self.chunk - 1) // self.chunk)
-        n_blocks = int(blk[k])
         nbytes = 48 * k + 4 * (k + 1)
+        host = self._pinned[s * self._slot_bytes:s * self._slot_bytes + nbytes]
+        raw = host.numpy()
+        raw[:48 * k] = tab.view(np.uint8)
+        raw[48 * k:] = blk.view(np.uint8)
+        n_blocks = int(blk[k])
         dev = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        dev.copy_(host[:nbytes], non_blocking=True)
+        dev.copy_(host, non_blocking=True)
         ev = self._events[s]
         if ev is None:
             ev = self._events[s] = torch.cuda.Event()
@@ -206,19 +212,15 @@ class FusedClipSGD:
         base = dev.data_ptr()
         if by_norm:
             ng = len(self.optimizers)
-            border = np.searchsorted(owner, np.arange(ng + 1)).astype(np.int32)   # the table is ordered by optimizer
-            border_blk = blk[border]
             norms = torch.empty(ng, dtype=torch.float32, device=device)
             ws = torch.empty(lib.lgd_sgd_norm_ws_bytes(ng), dtype=torch.uint8, device=device)
-            hip.check(lib.lgd_sgd_norm_step(ctypes.c_void_p(base), ctypes.c_void_p(base + 48 * k), k, n_blocks, ctypes.c_void_p(border.ctypes.data),
-                                            ctypes.c_void_p(border_blk.ctypes.data), ng, _norm_code(self.norm_type), ctypes.c_float(float(self.clip_norm)),
-                                            hip.ptr(ws), hip.ptr(norms), hip.stream_ptr()), "lgd_sgd_norm_step")
+            hip.check(lib.lgd_sgd_norm_step(base, base + 48 * k, k, n_blocks, border.ctypes.data, border_blk.ctypes.data, ng, _norm_code(self.norm_type),
+                                            float(self.clip_norm), ws.data_ptr(), norms.data_ptr(), hip.stream_ptr()), "lgd_sgd_norm_step")
             self.total_norms = norms
         else:
-            hip.check(lib.lgd_sgd_clip_step(ctypes.c_void_p(base), ctypes.c_void_p(base + 48 * k), k, n_blocks,
-                                            ctypes.c_float(self.clip_value), hip.stream_ptr()), "lgd_sgd_clip_step")
+            hip.check(lib.lgd_sgd_clip_step(base, base + 48 * k, k, n_blocks, self.clip_value, hip.stream_ptr()), "lgd_sgd_clip_step")
         # the kernel wrote p, g and the momentum buffers through raw pointers: tell autograd's version counters, which the fold
         # caches (ConvBN._frozen_fold, FrozenBatchNorm2d.scale_shift) key on and the saved-tensor check reads
-        torch.autograd.graph.increment_version([params[i] for i in idx] + [grads[i] for i in idx] + [self._m_ref[i] for i in idx])
+        torch.autograd.graph.increment_version(params + grads + [self._m_ref[i] for i in idx])
         for o in self.optimizers:
             o._opt_called = True   # what the LR schedulers' "scheduler.step() before optimizer.step()" check looks at
