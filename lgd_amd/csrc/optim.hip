@@ -10,7 +10,8 @@
 //   buf <- mu buf + d                       (a zero-initialised buffer reproduces torch's first step, buf = d, exactly)
 //   p   <- p - lr buf
 // or, clipping by NORM (lgd_sgd_norm_step): the gradients of every optimizer are one vector, g <- c g with c = min(1, max_norm / (norm + 1e-6)) of that
-// optimizer's norm; two launches more: partial sums over the same table (reads g once more) and one workgroup per optimizer that joins them.
+// optimizer's norm; one launch more: partial sums over the same table (reads g once more), which every workgroup of the update joins for itself while its own loads
+// are on their way.
 #include "grad_norm.h"
 
 #pragma clang fp contract(off)   // mu * buf + d keeps torch's two roundings (mul_ then add_); the fma calls below are explicit
@@ -42,9 +43,10 @@ template <bool NORM> __device__ __forceinline__ float sgd_clipped(float g, float
     return g < -clip ? -clip : (g > clip ? clip : g);
 }
 
-template <bool VEC, bool NORM>
-__device__ __forceinline__ void sgd_chunk(const lgd_sgd_tensor& t, long long base, float clip) {
-    const bool write_g = !NORM || clip != 1.f;   // a factor of 1 leaves the gradients as they are
+// clip_of(): the clamp's bound, or (NORM) the optimizer's factor; all threads call it once, behind the vector loads
+template <bool VEC, bool NORM, typename Clip>
+__device__ __forceinline__ void sgd_chunk(const lgd_sgd_tensor& t, long long base, Clip clip_of) {
+    float clip;
     const float lr = t.lr, wd = t.wd, mu = t.mu;
     if constexpr (VEC) {
         float4 p[4], g[4], m[4];
@@ -59,6 +61,8 @@ __device__ __forceinline__ void sgd_chunk(const lgd_sgd_tensor& t, long long bas
                 g[k] = make_float4(gv.x, gv.y, gv.z, gv.w);
             }
         }
+        clip = clip_of();
+        const bool write_g = !NORM || clip != 1.f;   // a factor of 1 leaves the gradients as they are
         #pragma unroll
         for (int k = 0; k < 4; ++k) {
             if (!on[k]) continue;
@@ -76,7 +80,10 @@ __device__ __forceinline__ void sgd_chunk(const lgd_sgd_tensor& t, long long bas
             if (write_g) sgd_storeu(t.g + i, go);
             sgd_store4(t.m + i, m[k]);
         }
+    } else {
+        clip = clip_of();
     }
+    const bool write_g = !NORM || clip != 1.f;
     // scalar path: parameters / momentum buffers that are not 16-byte aligned (never torch's own allocations), and the < 4-element
     // tail of a vector chunk
     const long long end = base + kSgdChunk < t.n ? base + kSgdChunk : t.n;
@@ -100,24 +107,45 @@ __device__ __forceinline__ int sgd_tensor_of(const int32_t* __restrict__ blk_off
     return lo;
 }
 
-template <bool NORM>
-__global__ __launch_bounds__(256) void sgd_clip_kernel(const lgd_sgd_tensor* __restrict__ tab, const int32_t* __restrict__ blk_off,
-                                                        int nt, float clip, const float* __restrict__ coef) {
-    const int lo = sgd_tensor_of(blk_off, 0, nt, (int)blockIdx.x);
-    const lgd_sgd_tensor t = tab[lo];
-    const long long base = (long long)((int)blockIdx.x - blk_off[lo]) * kSgdChunk;
-    if (base >= t.n) return;
-    const bool vec = ((reinterpret_cast<uintptr_t>(t.p) | reinterpret_cast<uintptr_t>(t.m)) & 15) == 0 && (reinterpret_cast<uintptr_t>(t.g) & 3) == 0;
-    if (NORM) clip = coef[t.reserved];
-    if (vec) sgd_chunk<true, NORM>(t, base, clip);
-    else sgd_chunk<false, NORM>(t, base, clip);
-}
-
 constexpr int kSgdNormGrid = 512;   // workgroups per optimizer: one partial word each
 struct SgdGroups {
     int tensor[LGD_MAX_SGD_GROUPS + 1];   // borders in the table
     int blk[LGD_MAX_SGD_GROUPS + 1];      // and in its blocks
+    int n;
 };
+
+__device__ __forceinline__ bool sgd_vec(const lgd_sgd_tensor& t) {
+    return ((reinterpret_cast<uintptr_t>(t.p) | reinterpret_cast<uintptr_t>(t.m)) & 15) == 0 && (reinterpret_cast<uintptr_t>(t.g) & 3) == 0;
+}
+
+__global__ __launch_bounds__(256) void sgd_clip_kernel(const lgd_sgd_tensor* __restrict__ tab, const int32_t* __restrict__ blk_off, int nt, float clip) {
+    const int lo = sgd_tensor_of(blk_off, 0, nt, (int)blockIdx.x);
+    const lgd_sgd_tensor t = tab[lo];
+    const long long base = (long long)((int)blockIdx.x - blk_off[lo]) * kSgdChunk;
+    if (base >= t.n) return;
+    if (sgd_vec(t)) sgd_chunk<true, false>(t, base, [&] { return clip; });
+    else sgd_chunk<false, false>(t, base, [&] { return clip; });
+}
+
+// the update with the gradients clipped by their optimizer's norm, of which `part` holds kSgdNormGrid partial words per group
+template <int NT>
+__global__ __launch_bounds__(256) void sgd_norm_step_kernel(const lgd_sgd_tensor* __restrict__ tab, const int32_t* __restrict__ blk_off, SgdGroups g,
+                                                             const double* __restrict__ part, float max_norm, float* __restrict__ norms) {
+    __shared__ double sh[4];
+    if (blockIdx.x == 0 && (int)threadIdx.x < g.n && g.blk[threadIdx.x] == g.blk[threadIdx.x + 1]) norms[threadIdx.x] = 0.f;   // groups without an element
+    if ((int)blockIdx.x >= g.blk[g.n]) return;
+    const int lo = sgd_tensor_of(blk_off, 0, g.tensor[g.n], (int)blockIdx.x);
+    const lgd_sgd_tensor t = tab[lo];
+    const long long base = (long long)((int)blockIdx.x - blk_off[lo]) * kSgdChunk;
+    const auto factor = [&] {
+        const int k = t.reserved;
+        const float v = norm_total<NT>(part + (size_t)k * kSgdNormGrid, kSgdNormGrid, sh);
+        if ((int)blockIdx.x == g.blk[k] && threadIdx.x == 0) norms[k] = v;
+        return norm_coef(v, max_norm);
+    };
+    if (sgd_vec(t)) sgd_chunk<true, true>(t, base, factor);
+    else sgd_chunk<false, true>(t, base, factor);
+}
 
 // partial norms of the gradients of group blockIdx.y; its workgroups sweep the group's blocks side by side.  Plain loads: what fits stays in the caches
 // for the update's read
@@ -137,23 +165,13 @@ __global__ __launch_bounds__(256) void sgd_norm_kernel(const lgd_sgd_tensor* __r
     if (threadIdx.x == 0) part[k * kSgdNormGrid + blockIdx.x] = acc.word();
 }
 
-// one workgroup per group: its norm and its factor
 template <int NT>
-__global__ __launch_bounds__(256) void sgd_coef_kernel(const double* __restrict__ part, float max_norm, float* __restrict__ norms, float* __restrict__ coef) {
-    __shared__ double sh[4];
-    const float v = norm_total<NT>(part + blockIdx.x * kSgdNormGrid, kSgdNormGrid, sh);
-    if (threadIdx.x == 0) { norms[blockIdx.x] = v; coef[blockIdx.x] = norm_coef(v, max_norm); }
-}
-
-template <int NT>
-static int sgd_norm_run(const lgd_sgd_tensor* table, const int32_t* blk_off, int n_tensors, int n_blocks, const SgdGroups& g, int n_groups, float max_norm,
-                        void* ws, float* norms, hipStream_t s) {
+static int sgd_norm_run(const lgd_sgd_tensor* table, const int32_t* blk_off, const SgdGroups& g, float max_norm, void* ws, float* norms, hipStream_t s) {
     double* part = static_cast<double*>(ws);
-    float* coef = reinterpret_cast<float*>(part + (size_t)n_groups * kSgdNormGrid);
-    LGD_LAUNCH("sgd_norm_kernel", sgd_norm_kernel<NT>, dim3(kSgdNormGrid, (unsigned)n_groups), dim3(256), 0, s, table, blk_off, g, part);
-    LGD_LAUNCH("sgd_coef_kernel", sgd_coef_kernel<NT>, dim3((unsigned)n_groups), dim3(256), 0, s, part, max_norm, norms, coef);
-    if (n_blocks > 0)
-        LGD_LAUNCH("sgd_norm_step_kernel", sgd_clip_kernel<true>, dim3((unsigned)n_blocks), dim3(256), 0, s, table, blk_off, n_tensors, 0.f, coef);
+    const int n_blocks = g.blk[g.n];
+    LGD_LAUNCH("sgd_norm_kernel", sgd_norm_kernel<NT>, dim3(kSgdNormGrid, (unsigned)g.n), dim3(256), 0, s, table, blk_off, g, part);
+    LGD_LAUNCH("sgd_norm_step_kernel", sgd_norm_step_kernel<NT>, dim3(n_blocks < 1 ? 1u : (unsigned)n_blocks), dim3(256), 0, s, table, blk_off, g,
+               (const double*)part, max_norm, norms);
     return check_launch();
 }
 
@@ -165,13 +183,13 @@ int lgd_sgd_chunk_elems(void) { return lgd::kSgdChunk; }
 
 int lgd_sgd_clip_step(const lgd_sgd_tensor* table, const int32_t* blk_off, int n_tensors, int n_blocks, float clip_value, void* stream) {
     if (!table || !blk_off || n_tensors < 1 || n_blocks < 1 || !(clip_value > 0.f)) return LGD_EINVAL;
-    LGD_LAUNCH("sgd_clip_kernel", lgd::sgd_clip_kernel<false>, dim3((unsigned)n_blocks), dim3(256), 0, (hipStream_t)stream, table, blk_off,
-               n_tensors, clip_value, (const float*)nullptr);
+    LGD_LAUNCH("sgd_clip_kernel", lgd::sgd_clip_kernel, dim3((unsigned)n_blocks), dim3(256), 0, (hipStream_t)stream, table, blk_off,
+               n_tensors, clip_value);
     return lgd::check_launch();
 }
 
 size_t lgd_sgd_norm_ws_bytes(int n_groups) {
-    return n_groups < 1 ? 0 : (size_t)n_groups * (lgd::kSgdNormGrid * sizeof(double) + sizeof(float));
+    return n_groups < 1 ? 0 : (size_t)n_groups * lgd::kSgdNormGrid * sizeof(double);
 }
 
 int lgd_sgd_norm_step(const lgd_sgd_tensor* table, const int32_t* blk_off, int n_tensors, int n_blocks, const int32_t* group_off_host,
@@ -180,15 +198,16 @@ int lgd_sgd_norm_step(const lgd_sgd_tensor* table, const int32_t* blk_off, int n
         !(max_norm >= 0.f) || !ws || !norms_out)
         return LGD_EINVAL;
     lgd::SgdGroups g = {};
+    g.n = n_groups;
     for (int k = 0; k <= n_groups; ++k) {
         g.tensor[k] = group_off_host[k]; g.blk[k] = group_blk_host[k];
         if (k > 0 && (g.tensor[k] < g.tensor[k - 1] || g.blk[k] < g.blk[k - 1] || (g.tensor[k] == g.tensor[k - 1] && g.blk[k] != g.blk[k - 1]))) return LGD_EINVAL;
     }
     if (g.tensor[0] != 0 || g.blk[0] != 0 || g.tensor[n_groups] != n_tensors || g.blk[n_groups] != n_blocks) return LGD_EINVAL;
     hipStream_t s = (hipStream_t)stream;
-    if (norm_type == LGD_NORM_2) return lgd::sgd_norm_run<LGD_NORM_2>(table, blk_off, n_tensors, n_blocks, g, n_groups, max_norm, ws, norms_out, s);
-    if (norm_type == LGD_NORM_1) return lgd::sgd_norm_run<LGD_NORM_1>(table, blk_off, n_tensors, n_blocks, g, n_groups, max_norm, ws, norms_out, s);
-    if (norm_type == LGD_NORM_INF) return lgd::sgd_norm_run<LGD_NORM_INF>(table, blk_off, n_tensors, n_blocks, g, n_groups, max_norm, ws, norms_out, s);
+    if (norm_type == LGD_NORM_2) return lgd::sgd_norm_run<LGD_NORM_2>(table, blk_off, g, max_norm, ws, norms_out, s);
+    if (norm_type == LGD_NORM_1) return lgd::sgd_norm_run<LGD_NORM_1>(table, blk_off, g, max_norm, ws, norms_out, s);
+    if (norm_type == LGD_NORM_INF) return lgd::sgd_norm_run<LGD_NORM_INF>(table, blk_off, g, max_norm, ws, norms_out, s);
     return LGD_EINVAL;
 }
 
