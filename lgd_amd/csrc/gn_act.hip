@@ -17,11 +17,14 @@
 
 namespace lgd {
 
-constexpr int kGaWorkgroups = 1024;    // of the streaming kernels, about: 4 per CU (768 and 2048: up to 10 and 40 % slower)
+// Workgroups of a streaming call, about: two for every CU, in step.  8 x 320 x 256 x 256 bf16, forward / backward us: 512 168 / 291, 768 197 / 345 (three on
+// some CUs, four on others), 1024 177 / 299
+constexpr int kGaWorkgroups = 512;
 constexpr int kGaU = 4, kGaUB = 2;     // vectors (of x; of x and dy each) of a thread in flight
-constexpr int kGaThreads = 256;
+constexpr int kGaThreads = 256;        // of the kernels in between
+constexpr int kGaMax = 320;            // of the streaming kernels: 192, 256 or 320, whichever has a vector for most of its threads
 constexpr int kGaFusedG = 512;         // groups of a fused call at most (its statistics lie in LDS) ...
-constexpr int kGaFusedRecords = 4096;  // ... and records x groups of a sample (64 KB that every workgroup of the apply kernel reads from the L2)
+constexpr int kGaFusedRecords = 8192;  // ... and records x groups of a sample (64 - 128 KB that every workgroup of the apply kernel reads from the L2)
 
 struct GaArgs {
     const void* x[LGD_MAX_LEVELS];
@@ -33,16 +36,16 @@ struct GaArgs {
     int wg0[LGD_MAX_LEVELS + 1];     // first workgroup of the map: B * K per map
     int L, B, C, G, cg;
     int P, PV;                       // super-row: elements, vectors
+    int NT;                          // threads of a workgroup
     int cols, R, nCB;                // vectors of a column block, super-rows a workgroup covers at once, column blocks
-    int whole;                       // column blocks hold whole groups (a single one always does)
-    int W;                           // width of a chunk's record in `part`: whole: G (forward), C (backward); otherwise P
+    int mixed;                       // several column blocks that cut groups or rows: each leaves records of its own, of all groups and channels
     double eps;
     const void* gamma;               // [C] or null
     const void* beta;
     int ptype;                       // LGD_F32 / LGD_BF16 / LGD_F16
-    double* partd;                   // forward [chunk][W][2]
-    float* partf;                    // backward [chunk][W][2]
-    float* partg;                    // backward, fused: [chunk][G][2], the channel sums with gamma, by group
+    double* partd;                   // forward [record][G][2], a record per chunk (mixed: and column block)
+    float* partf;                    // backward [record][C][2]
+    float* partg;                    // backward, fused: [record][G][2], the channel sums with gamma, by group
     int fused;                       // the apply kernels reduce the records themselves (no kernel in between)
     int nparam;                      // fused backward: workgroups in front of the apply kernel's own that make dgamma and dbeta
     double* stats;                   // [L*B*G][2] mean, rstd
@@ -62,17 +65,23 @@ template <typename T> __device__ __forceinline__ void ga_store(T* p, const lgd_u
     __builtin_nontemporal_store((typename GaU<sizeof(T)>::type)u, reinterpret_cast<typename GaU<sizeof(T)>::type*>(p));
 }
 
-// the channels and groups of a column block (whole ones only)
-struct GaBlock { int c0, nc, g0, ng; };
+// The channels and groups that a column block's record holds: its own where blocks are whole groups, otherwise (one block, or mixed) all.  Position o of
+// the block (element p0 + o of the super-row) is channel (p0 + o) % C: first(c) is the first position of channel c, the others follow in steps of C
+struct GaBlock {
+    int c0, nc, g0, ng, np, shift, C;
+    __device__ __forceinline__ int first(int c) const { const int o = c - shift; return o < 0 ? o + C : o; }
+};
 template <int V> __device__ __forceinline__ GaBlock ga_block(const GaArgs& a) {
-    GaBlock q = {0, a.C, 0, a.G};
-    if (a.nCB > 1) {
-        q.c0 = blockIdx.y * a.cols * V;
-        q.nc = min(a.cols * V, a.C - q.c0);
+    const int p0 = blockIdx.y * a.cols * V;
+    GaBlock q = {0, a.C, 0, a.G, min(a.cols * V, a.P - p0), p0 % a.C, a.C};
+    if (a.nCB > 1 && !a.mixed) {
+        q.c0 = p0; q.nc = q.np;
         q.g0 = q.c0 / a.cg; q.ng = q.nc / a.cg;
     }
     return q;
 }
+__device__ __forceinline__ int ga_per_chunk(const GaArgs& a) { return a.mixed ? a.nCB : 1; }   // records of a chunk
+__device__ __forceinline__ size_t ga_record(const GaArgs& a) { return a.mixed ? (size_t)blockIdx.x * a.nCB + blockIdx.y : blockIdx.x; }
 
 struct GaWhere { int l, b, k; };
 __device__ __forceinline__ GaWhere ga_locate(const GaArgs& a, int w) {
@@ -99,50 +108,36 @@ __device__ __forceinline__ GaThread ga_thread(const GaArgs& a, int E) {
     return t;
 }
 
-// the loads of a thread's first block, when it is whole (kernels that have something to compute first issue them in front of it)
-template <int V, int U, typename Regs> struct GaFirst {
+// A thread's way through its vectors, U in flight: begin() issues the first block's loads (kernels that have something to compute first call it in
+// front of that), run() consumes them and goes on.  load(e): a whole vector's registers; use(regs, e, count); part(e, count): the one vector that the
+// sample's end cuts, zero filled, comes last
+template <int V, int U, typename Regs> struct GaWalk {
+    int s, K, block, step, send;
+    unsigned e;   // element offset of super-row s (wraps only behind the last one, where it is not used)
     Regs v[U];
-    bool have;
-    template <typename Load> __device__ __forceinline__ void issue(const GaArgs& a, const GaWhere& q, const GaThread& t, Load load) {
-        const int s = q.k * U * a.R + t.r;
-        have = t.on && s + (U - 1) * a.R < t.send;
-        if (have) {
-            const unsigned e = (unsigned)s * a.P + t.v * V;
+    template <typename Load> __device__ __forceinline__ void loads(const GaArgs& a, Load load) {
+        #pragma unroll
+        for (int u = 0; u < U; ++u) if (s + u * a.R < send) v[u] = load(e + u * step);
+    }
+    template <typename Load> __device__ __forceinline__ void begin(const GaArgs& a, const GaWhere& q, const GaThread& t, Load load) {
+        K = a.K[q.l]; block = U * a.R; step = a.R * a.P; send = t.send;
+        s = q.k * block + t.r;
+        e = (unsigned)s * a.P + t.v * V;
+        loads(a, load);
+    }
+    template <typename Load, typename Part, typename Use>
+    __device__ __forceinline__ void run(const GaArgs& a, const GaWhere& q, const GaThread& t, int E, Load load, Part part, Use use) {
+        while (s < send) {
             #pragma unroll
-            for (int u = 0; u < U; ++u) v[u] = load(e + u * a.R * a.P);
+            for (int u = 0; u < U; ++u) if (s + u * a.R < send) use(v[u], e + u * step, V);
+            s += K * block; e += (unsigned)(K * U) * step;
+            loads(a, load);
         }
+        if (a.P == a.C || !t.on) return;   // samples are whole vectors
+        const unsigned cut = (unsigned)send * a.P + t.v * V;
+        if (cut < (unsigned)E && send / block % K == q.k && send % a.R == t.r) use(part(cut, E - cut), cut, E - cut);
     }
 };
-
-// every vector of the thread, U in flight; the (at most one) vector that the sample's end cuts comes with its count
-template <int V, int U, typename Regs, typename Load, typename Part, typename Use>
-__device__ __forceinline__ void ga_walk(const GaArgs& a, const GaWhere& q, const GaThread& t, int E, GaFirst<V, U, Regs>* first, Load load, Part part, Use use) {
-    if (!t.on) return;
-    const int block = U * a.R, K = a.K[q.l], step = a.R * a.P;
-    int s = q.k * block + t.r;
-    unsigned e = (unsigned)s * a.P + t.v * V;   // (wraps only behind the last super-row, where it is not used)
-    if (first && first->have) {
-        #pragma unroll
-        for (int u = 0; u < U; ++u) use(first->v[u], e + u * step, V);
-        s += K * block; e += (unsigned)(K * U) * step;
-    }
-    for (; s + (U - 1) * a.R < t.send; s += K * block, e += (unsigned)(K * U) * step) {
-        Regs v[U];
-        #pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = load(e + u * step);
-        #pragma unroll
-        for (int u = 0; u < U; ++u) use(v[u], e + u * step, V);
-    }
-    if (s > t.send) return;
-    Regs v[U];   // the thread's last block, cut by the sample's end
-    #pragma unroll
-    for (int u = 0; u < U; ++u) if (s + u * a.R < t.send) v[u] = load(e + u * step);
-    #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        if (s + u * a.R < t.send) use(v[u], e + u * step, V);
-        else if (s + u * a.R == t.send && e + u * step < (unsigned)E) use(part(e + u * step, E - e - u * step), e + u * step, E - e - u * step);
-    }
-}
 
 // the channels of the thread's V lanes and their groups, f(lane, channel, group) (one division for all of them)
 template <int V, typename F>
@@ -177,7 +172,7 @@ template <typename T> __device__ __forceinline__ void ga_store_n(T* p, const lgd
 }
 
 // ---- sums of a workgroup: every thread brings V pairs (one per position of the super-row); fixed-order tree over the R super-rows, result in
-// sh[position][2] for the positions of this column block.  sh holds kGaThreads * V pairs.
+// sh[position][2] for the positions of this column block.  sh holds kGaMax * V pairs.
 template <int V, typename A>
 __device__ __forceinline__ void ga_block_positions(const GaArgs& a, const GaThread& t, A (&s0)[V], A (&s1)[V], A* sh) {
     const int r = t.r, col = threadIdx.x - r * a.cols;
@@ -208,11 +203,11 @@ __device__ __forceinline__ void ga_block_positions(const GaArgs& a, const GaThre
 // sums over the n terms of each of ng groups: value(g, i, k) of term i, k in {0, 1}; put(2 g + k, sum).  Few groups are split over the workgroup (a
 // thread walking a whole group alone took 12 us at 512 channels), the parts meet in a tree.  Barriers inside
 template <typename Value, typename Put>
-__device__ __forceinline__ void ga_block_groups(int ng, int n, Value value, Put put) {
-    __shared__ double tmp[kGaThreads];
+__device__ __forceinline__ void ga_block_groups(int nt, int ng, int n, Value value, Put put) {
+    __shared__ double tmp[kGaMax];
     const int outs = 2 * ng;
-    if (outs > kGaThreads / 2) {
-        for (int j = threadIdx.x; j < outs; j += kGaThreads) {
+    if (outs > nt / 2) {
+        for (int j = threadIdx.x; j < outs; j += nt) {
             double s = 0.0;
             for (int i = 0; i < n; ++i) s += value(j >> 1, i, j & 1);
             put(j, s);
@@ -220,7 +215,7 @@ __device__ __forceinline__ void ga_block_groups(int ng, int n, Value value, Put 
         return;
     }
     int slices = 1;
-    while (2 * slices * outs <= kGaThreads) slices <<= 1;
+    while (2 * slices * outs <= nt) slices <<= 1;
     const int sl = threadIdx.x / outs, j = threadIdx.x - sl * outs;
     double s = 0.0;
     if (sl < slices) for (int i = sl; i < n; i += slices) s += value(j >> 1, i, j & 1);
@@ -234,17 +229,20 @@ __device__ __forceinline__ void ga_block_groups(int ng, int n, Value value, Put 
 }
 
 template <typename T, bool UG>
-__global__ __launch_bounds__(kGaThreads) void ga_stats_kernel(GaArgs a) {
+__global__ __launch_bounds__(kGaMax) void ga_stats_kernel(GaArgs a) {
     constexpr int V = Vec16<T>::V, S = UG ? 1 : V;
-    __shared__ double sh[kGaThreads * S * 2];
+    __shared__ double sh[kGaMax * S * 2];
     const GaWhere q = ga_locate(a, blockIdx.x);
     const int E = a.E[q.l];
     const GaThread t = ga_thread<V>(a, E);
     const T* __restrict__ px = static_cast<const T*>(a.x[q.l]) + (size_t)q.b * E;
+    const auto load = [&](unsigned e) { return GaX<T>{ga_load(px + e)}; };
+    GaWalk<V, kGaU, GaX<T>> walk;
+    walk.begin(a, q, t, load);
     double s0[S], s1[S];
     #pragma unroll
     for (int i = 0; i < S; ++i) s0[i] = s1[i] = 0.0;
-    ga_walk<V, kGaU, GaX<T>>(a, q, t, E, (GaFirst<V, kGaU, GaX<T>>*)nullptr, [&](unsigned e) { return GaX<T>{ga_load(px + e)}; },
+    walk.run(a, q, t, E, load,
         [&](unsigned e, int n) { return GaX<T>{ga_load_part(px + e, n)}; },
         [&](const GaX<T>& v, unsigned, int) {
             float f[V];
@@ -252,31 +250,23 @@ __global__ __launch_bounds__(kGaThreads) void ga_stats_kernel(GaArgs a) {
             #pragma unroll
             for (int i = 0; i < V; ++i) { const double d = f[i]; s0[UG ? 0 : i] += d; s1[UG ? 0 : i] = fma(d, d, s1[UG ? 0 : i]); }
         });
-    double* part = a.partd + (size_t)blockIdx.x * a.W * 2;
-    if constexpr (UG) {   // (whole column blocks) a thread's vectors lie in one group: its pair is all that the others need of it
+    double* part = a.partd + ga_record(a) * a.G * 2;
+    const GaBlock blk = ga_block<V>(a);
+    if constexpr (UG) {   // (not mixed) a thread's vectors lie in one group: its pair is all that the others need of it
         sh[2 * threadIdx.x] = s0[0]; sh[2 * threadIdx.x + 1] = s1[0];
         __syncthreads();
-        const GaBlock blk = ga_block<V>(a);
         const int per = a.cg / V;
-        ga_block_groups(blk.ng, a.R * per, [&](int g, int i, int k) {
+        ga_block_groups(a.NT, blk.ng, a.R * per, [&](int g, int i, int k) {
             const int r = i / per;
             return sh[2 * (r * a.cols + g * per + i - r * per) + k];
         }, [&](int j, double s) { part[2 * blk.g0 + j] = s; });
     } else {
         ga_block_positions<V, double>(a, t, s0, s1, sh);
-        if (a.whole) {   // positions -> groups
-            const int wraps = a.nCB == 1 ? a.P / a.C : 1;
-            const GaBlock blk = ga_block<V>(a);
-            ga_block_groups(blk.ng, a.cg, [&](int g, int i, int k) {
-                const int c = g * a.cg + i;
-                double s = sh[2 * c + k];
-                for (int w = 1; w < wraps; ++w) s += sh[2 * (w * a.C + c) + k];
-                return s;
-            }, [&](int j, double s) { part[2 * blk.g0 + j] = s; });
-        } else {
-            const int p0 = blockIdx.y * a.cols * V, np = min(a.cols * V, a.P - p0);
-            for (int j = threadIdx.x; j < 2 * np; j += kGaThreads) part[2 * (size_t)p0 + j] = sh[j];
-        }
+        ga_block_groups(a.NT, blk.ng, a.cg, [&](int g, int i, int k) {   // positions -> groups
+            double s = 0.0;
+            for (int o = blk.first((blk.g0 + g) * a.cg + i); o < blk.np; o += a.C) s += sh[2 * o + k];
+            return s;
+        }, [&](int j, double s) { part[2 * blk.g0 + j] = s; });
     }
 }
 
@@ -292,15 +282,10 @@ __device__ __forceinline__ void ga_moments(double s0, double s1, double n, doubl
 __global__ __launch_bounds__(kGaThreads) void ga_finalize_kernel(GaArgs a) {
     __shared__ double sh[4][2];
     const int seg = blockIdx.x, g = seg % a.G, lb = seg / a.G, l = lb / a.B, b = lb % a.B;
-    const int K = a.K[l], per = a.whole ? 1 : a.cg, wraps = a.whole ? 1 : a.W / a.C;
-    const double* p = a.partd + (size_t)(a.wg0[l] + b * K) * a.W * 2;
+    const int n = a.K[l] * ga_per_chunk(a);
+    const double2* p = reinterpret_cast<const double2*>(a.partd) + (size_t)(a.wg0[l] + b * a.K[l]) * ga_per_chunk(a) * a.G + g;
     double s0 = 0.0, s1 = 0.0;
-    const int n = K * per * wraps;
-    for (int i = threadIdx.x; i < n; i += kGaThreads) {
-        const int k = i / (per * wraps), j = i % (per * wraps);
-        const double* v = p + 2 * ((size_t)k * a.W + (j / per) * a.C + g * per + j % per);
-        s0 += v[0]; s1 += v[1];
-    }
+    for (int i = threadIdx.x; i < n; i += kGaThreads) { const double2 v = p[(size_t)i * a.G]; s0 += v.x; s1 += v.y; }
     s0 = wave_sum(s0); s1 = wave_sum(s1);
     if ((threadIdx.x & 63) == 0) { sh[threadIdx.x >> 6][0] = s0; sh[threadIdx.x >> 6][1] = s1; }
     __syncthreads();
@@ -312,16 +297,16 @@ __global__ __launch_bounds__(kGaThreads) void ga_finalize_kernel(GaArgs a) {
 // sums of the K records of G pairs of one sample, by every workgroup that needs them: put(g, s0, s1).  Threads = groups x slices of the records; the
 // slices meet in LDS, in a fixed order.  P2: pair of the records.  Barriers inside
 template <typename P2, typename Put>
-__device__ __forceinline__ void ga_records(const P2* __restrict__ p, int K, int G, const GaBlock& blk, Put put) {
-    __shared__ double tmp[kGaThreads][2];
+__device__ __forceinline__ void ga_records(int nt, const P2* __restrict__ p, int K, int G, const GaBlock& blk, Put put) {
+    __shared__ double tmp[kGaMax][2];
     int sub = 1;
-    while (sub < blk.ng && sub < kGaThreads) sub <<= 1;
-    const int slices = kGaThreads / sub, sl = threadIdx.x / sub;
+    while (sub < blk.ng && 2 * sub <= nt) sub <<= 1;
+    const int slices = nt / sub, sl = threadIdx.x / sub;
     const int gend = blk.g0 + blk.ng;
     for (int g0 = blk.g0; g0 < gend; g0 += sub) {
         const int g = g0 + (threadIdx.x & (sub - 1));
         double s0 = 0.0, s1 = 0.0;
-        if (g < gend) {
+        if (g < gend && sl < slices) {
             int k = sl;
             for (; k + 3 * slices < K; k += 4 * slices) {
                 P2 v[4];
@@ -343,26 +328,28 @@ __device__ __forceinline__ void ga_records(const P2* __restrict__ p, int K, int 
 }
 
 template <typename T, int ACT>
-__global__ __launch_bounds__(kGaThreads) void ga_apply_kernel(GaArgs a) {
+__global__ __launch_bounds__(kGaMax) void ga_apply_kernel(GaArgs a) {
     constexpr int V = Vec16<T>::V;
     const GaWhere q = ga_locate(a, blockIdx.x);
     const int E = a.E[q.l];
     const GaThread t = ga_thread<V>(a, E);
     const T* __restrict__ px = static_cast<const T*>(a.x[q.l]) + (size_t)q.b * E;
     T* __restrict__ po = static_cast<T*>(a.out[q.l]) + (size_t)q.b * E;
-    GaFirst<V, kGaU, GaX<T>> first;
-    first.issue(a, q, t, [&](unsigned e) { return GaX<T>{ga_stream(px + e)}; });
+    const auto load = [&](unsigned e) { return GaX<T>{ga_stream(px + e)}; };
+    GaWalk<V, kGaU, GaX<T>> walk;
+    walk.begin(a, q, t, load);
     double A[V], Bc[V];
     double* gst = a.stats + 2 * (size_t)(q.l * a.B + q.b) * a.G;
     const double* st = gst;
     if (a.fused) {   // the statistics from the chunks' records; the sample's first workgroup leaves them for the backward
         __shared__ double sst[2 * kGaFusedG];
         const double n = (double)a.HW[q.l] * a.cg;
-        ga_records(reinterpret_cast<const double2*>(a.partd) + (size_t)(a.wg0[q.l] + q.b * a.K[q.l]) * a.G, a.K[q.l], a.G, ga_block<V>(a), [&](int g, double s0, double s1) {
+        const int rec = ga_per_chunk(a);
+        ga_records(a.NT, reinterpret_cast<const double2*>(a.partd) + (size_t)(a.wg0[q.l] + q.b * a.K[q.l]) * rec * a.G, a.K[q.l] * rec, a.G, ga_block<V>(a), [&](int g, double s0, double s1) {
             double m, r;
             ga_moments(s0, s1, n, a.eps, m, r);
             sst[2 * g] = m; sst[2 * g + 1] = r;
-            if (q.k == 0) { gst[2 * g] = m; gst[2 * g + 1] = r; }
+            if (q.k == 0 && (!a.mixed || blockIdx.y == 0)) { gst[2 * g] = m; gst[2 * g + 1] = r; }
         });
         __syncthreads();
         st = sst;
@@ -371,12 +358,12 @@ __global__ __launch_bounds__(kGaThreads) void ga_apply_kernel(GaArgs a) {
         A[i] = st[2 * g + 1] * (double)ga_param(a.gamma, a.ptype, c, 1.f);
         Bc[i] = fma(-st[2 * g], A[i], (double)ga_param(a.beta, a.ptype, c, 0.f));
     });
-    ga_walk<V, kGaU, GaX<T>>(a, q, t, E, &first, [&](unsigned e) { return GaX<T>{ga_stream(px + e)}; }, [&](unsigned e, int n) { return GaX<T>{ga_load_part(px + e, n)}; },
+    walk.run(a, q, t, E, load, [&](unsigned e, int n) { return GaX<T>{ga_load_part(px + e, n)}; },
         [&](const GaX<T>& v, unsigned e, int n) {
             float f[V];
             Vec16<T>::unpack(v.x, f);
             #pragma unroll
-            for (int i = 0; i < V; ++i) f[i] = ga_act<ACT>((float)fma((double)f[i], A[i], Bc[i]));
+            for (int i = 0; i < V; ++i) f[i] = ga_act<ACT>(ga_single(fma((double)f[i], A[i], Bc[i])));
             ga_store_n(po + e, Vec16<T>::pack(f), n);
         });
 }
@@ -396,22 +383,23 @@ template <int V, bool UG> struct GaCoef {
 };
 
 template <typename T, int ACT, bool UG>
-__global__ __launch_bounds__(kGaThreads) void ga_bwd_stats_kernel(GaArgs a) {
+__global__ __launch_bounds__(kGaMax) void ga_bwd_stats_kernel(GaArgs a) {
     constexpr int V = Vec16<T>::V;
-    __shared__ float sh[kGaThreads * V * 2];
+    __shared__ float sh[kGaMax * V * 2];
     const GaWhere q = ga_locate(a, blockIdx.x);
     const int E = a.E[q.l];
     const GaThread t = ga_thread<V>(a, E);
     const T* __restrict__ px = static_cast<const T*>(a.x[q.l]) + (size_t)q.b * E;
     const T* __restrict__ pd = static_cast<const T*>(a.dy[q.l]) + (size_t)q.b * E;
-    GaFirst<V, kGaUB, GaXD<T>> first;
-    first.issue(a, q, t, [&](unsigned e) { return GaXD<T>{ga_load(px + e), ga_load(pd + e)}; });
+    const auto load = [&](unsigned e) { return GaXD<T>{ga_load(px + e), ga_load(pd + e)}; };
+    GaWalk<V, kGaUB, GaXD<T>> walk;
+    walk.begin(a, q, t, load);
     GaCoef<V, UG> k;
     k.fill(a, q, t);
     float s0[V], s1[V];
     #pragma unroll
     for (int i = 0; i < V; ++i) s0[i] = s1[i] = 0.f;
-    ga_walk<V, kGaUB, GaXD<T>>(a, q, t, E, &first, [&](unsigned e) { return GaXD<T>{ga_load(px + e), ga_load(pd + e)}; },
+    walk.run(a, q, t, E, load,
         [&](unsigned e, int n) { return GaXD<T>{ga_load_part(px + e, n), ga_load_part(pd + e, n)}; },
         [&](const GaXD<T>& v, unsigned, int) {
             float x[V], d[V];
@@ -423,24 +411,22 @@ __global__ __launch_bounds__(kGaThreads) void ga_bwd_stats_kernel(GaArgs a) {
             }
         });
     ga_block_positions<V, float>(a, t, s0, s1, sh);
-    float* part = a.partf + (size_t)blockIdx.x * a.W * 2;
-    if (a.whole) {   // positions -> channels, and with gamma -> groups
-        const int wraps = a.nCB == 1 ? a.P / a.C : 1;
-        const GaBlock blk = ga_block<V>(a);
-        for (int j = threadIdx.x; j < 2 * blk.nc; j += kGaThreads) {
-            float s = sh[j];
-            for (int w = 1; w < wraps; ++w) s += sh[2 * w * a.C + j];
-            part[2 * blk.c0 + j] = s;
-            sh[j] = s * ga_param(a.gamma, a.ptype, blk.c0 + (j >> 1), 1.f);   // (j is read and written by this thread only)
-        }
-        if (a.fused) {
-            float* gp = a.partg + (size_t)blockIdx.x * a.G * 2;
-            __syncthreads();
-            ga_block_groups(blk.ng, a.cg, [&](int g, int i, int k) { return (double)sh[2 * (g * a.cg + i) + k]; }, [&](int j, double s) { gp[2 * blk.g0 + j] = (float)s; });
-        }
-    } else {
-        const int p0 = blockIdx.y * a.cols * V, np = min(a.cols * V, a.P - p0);
-        for (int j = threadIdx.x; j < 2 * np; j += kGaThreads) part[2 * (size_t)p0 + j] = sh[j];
+    float* part = a.partf + ga_record(a) * a.C * 2;
+    const GaBlock blk = ga_block<V>(a);
+    for (int j = threadIdx.x; j < 2 * blk.nc; j += a.NT) {   // positions -> channels, and with gamma -> groups
+        const int c = blk.c0 + (j >> 1), k = j & 1, o0 = blk.first(c);
+        float s = 0.f;
+        for (int o = o0; o < blk.np; o += a.C) s += sh[2 * o + k];
+        part[2 * blk.c0 + j] = s;
+        if (o0 < blk.np) sh[2 * o0 + k] = s * ga_param(a.gamma, a.ptype, c, 1.f);   // (a channel's positions are read and written by this thread only)
+    }
+    if (a.fused) {
+        float* gp = a.partg + ga_record(a) * a.G * 2;
+        __syncthreads();
+        ga_block_groups(a.NT, blk.ng, a.cg, [&](int g, int i, int k) {
+            const int o = blk.first((blk.g0 + g) * a.cg + i);
+            return o < blk.np ? (double)sh[2 * o + k] : 0.0;
+        }, [&](int j, double s) { gp[2 * blk.g0 + j] = (float)s; });
     }
 }
 
@@ -450,8 +436,8 @@ __global__ __launch_bounds__(kGaThreads) void ga_bwd_stats_kernel(GaArgs a) {
 __global__ __launch_bounds__(256) void ga_bwd_finalize_kernel(GaArgs a) {
     __shared__ double sh[256][2];
     const int seg = blockIdx.x, g = seg % a.G, lb = seg / a.G, l = lb / a.B, b = lb % a.B, tid = threadIdx.x;
-    const int wraps = a.W / a.C, n = a.K[l] * wraps;
-    const float* p = a.partf + (size_t)(a.wg0[l] + b * a.K[l]) * a.W * 2;
+    const int n = a.K[l] * ga_per_chunk(a);
+    const float2* p = reinterpret_cast<const float2*>(a.partf) + (size_t)(a.wg0[l] + b * a.K[l]) * ga_per_chunk(a) * a.C;
     int sub = 1;
     while (sub < a.cg && sub < 256) sub <<= 1;
     double m1 = 0.0, m2 = 0.0;
@@ -459,7 +445,7 @@ __global__ __launch_bounds__(256) void ga_bwd_finalize_kernel(GaArgs a) {
         const int j = c0 + (tid & (sub - 1)), c = g * a.cg + j, slices = 256 / sub;
         double s0 = 0.0, s1 = 0.0;
         if (j < a.cg) {
-            auto at = [&](int i) { return reinterpret_cast<const float2*>(p)[(wraps == 1 ? (size_t)i * a.W : (size_t)(i / wraps) * a.W + (i % wraps) * a.C) + c]; };
+            auto at = [&](int i) { return p[(size_t)i * a.C + c]; };
             int i = tid / sub;
             for (; i + 3 * slices < n; i += 4 * slices) {
                 float2 v[4];
@@ -512,39 +498,39 @@ __global__ __launch_bounds__(256) void ga_param_kernel(GaArgs a) {
     }
 }
 
-// dgamma, dbeta of 16 channels: the channel sums of every chunk of every (map, sample); 16 channels x 16 slices of the records
+// dgamma, dbeta of 16 channels: the channel sums of every chunk of every (map, sample); 16 channels x NT / 16 slices of the records
 constexpr int kGaParamC = 16;
 __device__ __forceinline__ void ga_params(const GaArgs& a) {
-    __shared__ double sh[kGaThreads][2];
-    const int c = blockIdx.x * kGaParamC + (threadIdx.x & 15), sl = threadIdx.x >> 4, n = a.wg0[LGD_MAX_LEVELS];
+    __shared__ double sh[kGaMax][2];
+    const int c = blockIdx.x * kGaParamC + (threadIdx.x & 15), sl = threadIdx.x >> 4, slices = a.NT >> 4, n = a.wg0[LGD_MAX_LEVELS] * ga_per_chunk(a);
     const float2* __restrict__ p = reinterpret_cast<const float2*>(a.partf);
     double s0 = 0.0, s1 = 0.0;
     if (c < a.C) {
         int i = sl;
-        for (; i + 7 * 16 < n; i += 8 * 16) {
+        for (; i + 7 * slices < n; i += 8 * slices) {
             float2 v[8];
             #pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = p[(size_t)(i + u * 16) * a.C + c];
+            for (int u = 0; u < 8; ++u) v[u] = p[(size_t)(i + u * slices) * a.C + c];
             #pragma unroll
             for (int u = 0; u < 8; ++u) { s0 += (double)v[u].x; s1 += (double)v[u].y; }
         }
-        for (; i < n; i += 16) { const float2 v = p[(size_t)i * a.C + c]; s0 += (double)v.x; s1 += (double)v.y; }
+        for (; i < n; i += slices) { const float2 v = p[(size_t)i * a.C + c]; s0 += (double)v.x; s1 += (double)v.y; }
     }
     sh[threadIdx.x][0] = s0; sh[threadIdx.x][1] = s1;
     __syncthreads();
     if (sl == 0 && c < a.C) {
-        for (int i = 1; i < 16; ++i) { s0 += sh[threadIdx.x + 16 * i][0]; s1 += sh[threadIdx.x + 16 * i][1]; }
+        for (int i = 1; i < slices; ++i) { s0 += sh[threadIdx.x + 16 * i][0]; s1 += sh[threadIdx.x + 16 * i][1]; }
         if (a.dbeta) ga_param_store(a.dbeta, a.ptype, c, (float)s0);
         if (a.dgamma) ga_param_store(a.dgamma, a.ptype, c, (float)s1);
     }
 }
-__global__ __launch_bounds__(kGaThreads) void ga_params_kernel(GaArgs a) { ga_params(a); }
+__global__ __launch_bounds__(kGaMax) void ga_params_kernel(GaArgs a) { ga_params(a); }
 
 template <typename T, int ACT, bool UG>
-__global__ __launch_bounds__(kGaThreads) void ga_bwd_apply_kernel(GaArgs a) {
+__global__ __launch_bounds__(kGaMax) void ga_bwd_apply_kernel(GaArgs a) {
     constexpr int V = Vec16<T>::V;
     if ((int)blockIdx.x < a.nparam) {   // the first workgroups of a fused call: dgamma, dbeta out of all the chunks' channel sums
-        ga_params(a);
+        if (blockIdx.y == 0) ga_params(a);
         return;
     }
     const GaWhere q = ga_locate(a, blockIdx.x - a.nparam);
@@ -553,13 +539,15 @@ __global__ __launch_bounds__(kGaThreads) void ga_bwd_apply_kernel(GaArgs a) {
     const T* __restrict__ px = static_cast<const T*>(a.x[q.l]) + (size_t)q.b * E;
     const T* __restrict__ pd = static_cast<const T*>(a.dy[q.l]) + (size_t)q.b * E;
     T* __restrict__ po = static_cast<T*>(a.out[q.l]) + (size_t)q.b * E;
-    GaFirst<V, kGaUB, GaXD<T>> first;
-    first.issue(a, q, t, [&](unsigned e) { return GaXD<T>{ga_stream(px + e), ga_stream(pd + e)}; });
+    const auto load = [&](unsigned e) { return GaXD<T>{ga_stream(px + e), ga_stream(pd + e)}; };
+    GaWalk<V, kGaUB, GaXD<T>> walk;
+    walk.begin(a, q, t, load);
     const float* bs = a.bstats + 2 * (size_t)(q.l * a.B + q.b) * a.G;
     if (a.fused) {   // the two means from the chunks' records
         __shared__ float sbs[2 * kGaFusedG];
         const double n = (double)a.HW[q.l] * a.cg;
-        ga_records(reinterpret_cast<const float2*>(a.partg) + (size_t)(a.wg0[q.l] + q.b * a.K[q.l]) * a.G, a.K[q.l], a.G, ga_block<V>(a),
+        const int rec = ga_per_chunk(a);
+        ga_records(a.NT, reinterpret_cast<const float2*>(a.partg) + (size_t)(a.wg0[q.l] + q.b * a.K[q.l]) * rec * a.G, a.K[q.l] * rec, a.G, ga_block<V>(a),
                    [&](int g, double s0, double s1) { sbs[2 * g] = (float)(s0 / n); sbs[2 * g + 1] = (float)(s1 / n); });
         __syncthreads();
         bs = sbs;
@@ -570,7 +558,7 @@ __global__ __launch_bounds__(kGaThreads) void ga_bwd_apply_kernel(GaArgs a) {
     ga_lanes<V>(a, t, [&](int i, int, int g) {
         if (!UG || i == 0) { c2[UG ? 0 : i] = -k.at(i).r * bs[2 * g + 1]; c3[UG ? 0 : i] = -k.at(i).r * bs[2 * g]; }
     });
-    ga_walk<V, kGaUB, GaXD<T>>(a, q, t, E, &first, [&](unsigned e) { return GaXD<T>{ga_stream(px + e), ga_stream(pd + e)}; },
+    walk.run(a, q, t, E, load,
         [&](unsigned e, int n) { return GaXD<T>{ga_load_part(px + e, n), ga_load_part(pd + e, n)}; },
         [&](const GaXD<T>& v, unsigned e, int n) {
             float x[V], d[V];
@@ -594,19 +582,22 @@ static int ga_plan(GaArgs& a, const int32_t* hw, int L, int B, int C, int G, int
     a.L = L; a.B = B; a.C = C; a.G = G; a.cg = C / G;
     if (C > (1 << 26)) return LGD_EINVAL;
     a.P = C / ga_gcd(C, V) * V; a.PV = a.P / V;
-    a.nCB = (a.PV + kGaThreads - 1) / kGaThreads;
+    a.nCB = (a.PV + kGaMax - 1) / kGaMax;
     a.cols = (a.PV + a.nCB - 1) / a.nCB;
-    a.whole = a.nCB == 1;
-    if (!a.whole && a.P == C) {   // column blocks of whole groups, where one fits
-        const int unit = a.cg / ga_gcd(a.cg, V);   // vectors of lcm(cg, V) channels
-        if (unit <= kGaThreads) {
-            a.cols = (a.cols + unit - 1) / unit * unit;
-            if (a.cols > kGaThreads) a.cols = kGaThreads / unit * unit;
-            a.nCB = (a.PV + a.cols - 1) / a.cols;
-            a.whole = 1;
-        }
+    a.mixed = a.nCB > 1;
+    const int unit = a.cg / ga_gcd(a.cg, V);   // vectors of lcm(cg, V) channels: column blocks of whole groups, where one fits
+    if (a.mixed && a.P == C && unit <= kGaMax) {
+        a.cols = (a.cols + unit - 1) / unit * unit;
+        if (a.cols > kGaMax) a.cols = kGaMax / unit * unit;
+        a.nCB = (a.PV + a.cols - 1) / a.cols;
+        a.mixed = 0;
     }
-    a.R = kGaThreads / a.cols;
+    // threads: 256, or where that leaves more than a tenth without a vector, the width of which most have one (160 vectors a row: two rows for 320; 16 x 1280
+    // x 32 x 32 bf16 backward 49 us against 54).  240 of 256 stay: 320 took 4 % longer on 8 x 320 x 256 x 256
+    a.NT = kGaThreads;
+    for (int nt = 192; nt <= kGaMax && a.NT / a.cols * a.cols * 10 < a.NT * 9; nt += 64)
+        if (nt >= a.cols && nt / a.cols * a.cols * a.NT > a.NT / a.cols * a.cols * nt) a.NT = nt;
+    a.R = a.NT / a.cols;
     long long total = 0;
     for (int l = 0; l < L; ++l) {
         if (hw[2 * l] < 1 || hw[2 * l + 1] < 1) return LGD_EINVAL;
@@ -615,11 +606,10 @@ static int ga_plan(GaArgs& a, const int32_t* hw, int L, int B, int C, int G, int
         a.E[l] = (int)e; a.HW[l] = (int)n;
         total += e * B * size;
     }
-    long long bytes = total / kGaWorkgroups;
-    const long long least = total / 512 < 16384 ? 16384 : total / 512 > 32768 ? 32768 : total / 512;
-    if (bytes < least) bytes = least;
-    const long long block = 16LL * 4 * kGaThreads;   // (a block of U = 4 vectors a thread)
-    const long long cap = kGaFusedRecords / G;
+    const long long bytes = total / kGaWorkgroups < 16384 ? 16384 : total / kGaWorkgroups;
+    const long long block = 16LL * kGaU * a.R * a.cols;   // (U vectors a thread)
+    const int rec = a.mixed ? a.nCB : 1;
+    const long long cap = kGaFusedRecords / ((long long)G * rec);
     long long w = 0, wf = 0;
     for (int l = 0; l < L; ++l) {
         const long long sample = (long long)a.E[l] * size, want = (sample + bytes - 1) / bytes, most = (sample + block - 1) / block;
@@ -628,9 +618,9 @@ static int ga_plan(GaArgs& a, const int32_t* hw, int L, int B, int C, int G, int
         w += B * k;
         wf += B * (k < cap ? k : cap);
     }
-    if (w > 0x3fffffffLL || (long long)L * B * G > 0x7fffffffLL) return LGD_EINVAL;
+    if (w * rec > 0x3fffffffLL || (long long)L * B * G > 0x7fffffffLL) return LGD_EINVAL;
     // one kernel less where the records are few enough without leaving the chip short of workgroups
-    a.fused = a.whole && G <= kGaFusedG && cap >= 1 && (wf == w || wf >= 512);
+    a.fused = G <= kGaFusedG && cap >= 1 && (wf == w || wf >= 384);
     w = 0;
     for (int l = 0; l < L; ++l) {
         if (a.fused && a.K[l] > cap) a.K[l] = (int)cap;
@@ -643,34 +633,35 @@ static int ga_plan(GaArgs& a, const int32_t* hw, int L, int B, int C, int G, int
 
 static size_t ga_round(size_t n) { return (n + 255) & ~(size_t)255; }
 static size_t ga_chunks(const GaArgs& a) { return (size_t)a.wg0[LGD_MAX_LEVELS]; }
+static size_t ga_rows(const GaArgs& a) { return ga_chunks(a) * (size_t)(a.mixed ? a.nCB : 1); }   // records of a call
 
 template <typename T>
 static int ga_fwd(GaArgs& a, int act, hipStream_t s) {
     const dim3 grid((unsigned)ga_chunks(a), (unsigned)a.nCB);
-    if (a.whole && a.cg % Vec16<T>::V == 0) LGD_LAUNCH("gn_act_stats_kernel", (ga_stats_kernel<T, true>), grid, dim3(kGaThreads), 0, s, a);
-    else LGD_LAUNCH("gn_act_stats_kernel", (ga_stats_kernel<T, false>), grid, dim3(kGaThreads), 0, s, a);
+    if (!a.mixed && a.cg % Vec16<T>::V == 0) LGD_LAUNCH("gn_act_stats_kernel", (ga_stats_kernel<T, true>), grid, dim3((unsigned)a.NT), 0, s, a);
+    else LGD_LAUNCH("gn_act_stats_kernel", (ga_stats_kernel<T, false>), grid, dim3((unsigned)a.NT), 0, s, a);
     if (!a.fused) LGD_LAUNCH("gn_act_finalize_kernel", ga_finalize_kernel, dim3((unsigned)(a.L * a.B * a.G)), dim3(kGaThreads), 0, s, a);
-    if (act == kActNone) LGD_LAUNCH("gn_act_apply_kernel", (ga_apply_kernel<T, kActNone>), grid, dim3(kGaThreads), 0, s, a);
-    else if (act == kActRelu) LGD_LAUNCH("gn_act_apply_kernel", (ga_apply_kernel<T, kActRelu>), grid, dim3(kGaThreads), 0, s, a);
-    else LGD_LAUNCH("gn_act_apply_kernel", (ga_apply_kernel<T, kActSilu>), grid, dim3(kGaThreads), 0, s, a);
+    if (act == kActNone) LGD_LAUNCH("gn_act_apply_kernel", (ga_apply_kernel<T, kActNone>), grid, dim3((unsigned)a.NT), 0, s, a);
+    else if (act == kActRelu) LGD_LAUNCH("gn_act_apply_kernel", (ga_apply_kernel<T, kActRelu>), grid, dim3((unsigned)a.NT), 0, s, a);
+    else LGD_LAUNCH("gn_act_apply_kernel", (ga_apply_kernel<T, kActSilu>), grid, dim3((unsigned)a.NT), 0, s, a);
     return check_launch();
 }
 
 template <typename T, int ACT, bool UG>
 static int ga_bwd(GaArgs& a, hipStream_t s) {
     const dim3 grid((unsigned)ga_chunks(a), (unsigned)a.nCB);
-    LGD_LAUNCH("gn_act_bwd_stats_kernel", (ga_bwd_stats_kernel<T, ACT, UG>), grid, dim3(kGaThreads), 0, s, a);
+    LGD_LAUNCH("gn_act_bwd_stats_kernel", (ga_bwd_stats_kernel<T, ACT, UG>), grid, dim3((unsigned)a.NT), 0, s, a);
     const bool params = a.dgamma || a.dbeta;
     if (a.fused) {
         const unsigned np = params ? (unsigned)((a.C + kGaParamC - 1) / kGaParamC) : 0u;
         a.nparam = (int)np;
-        if (a.out[0]) LGD_LAUNCH("gn_act_bwd_apply_kernel", (ga_bwd_apply_kernel<T, ACT, UG>), dim3(grid.x + np), dim3(kGaThreads), 0, s, a);
-        else if (params) LGD_LAUNCH("gn_act_bwd_param_kernel", ga_params_kernel, dim3(np), dim3(kGaThreads), 0, s, a);
+        if (a.out[0]) LGD_LAUNCH("gn_act_bwd_apply_kernel", (ga_bwd_apply_kernel<T, ACT, UG>), dim3(grid.x + np, grid.y), dim3((unsigned)a.NT), 0, s, a);
+        else if (params) LGD_LAUNCH("gn_act_bwd_param_kernel", ga_params_kernel, dim3(np), dim3((unsigned)a.NT), 0, s, a);
         return check_launch();
     }
     LGD_LAUNCH("gn_act_bwd_finalize_kernel", ga_bwd_finalize_kernel, dim3((unsigned)(a.L * a.B * a.G)), dim3(256), 0, s, a);
     if (params) LGD_LAUNCH("gn_act_bwd_param_kernel", ga_param_kernel, dim3((unsigned)((a.C + 63) / 64)), dim3(256), 0, s, a);
-    if (a.out[0]) LGD_LAUNCH("gn_act_bwd_apply_kernel", (ga_bwd_apply_kernel<T, ACT, UG>), grid, dim3(kGaThreads), 0, s, a);
+    if (a.out[0]) LGD_LAUNCH("gn_act_bwd_apply_kernel", (ga_bwd_apply_kernel<T, ACT, UG>), grid, dim3((unsigned)a.NT), 0, s, a);
     return check_launch();
 }
 template <typename T, bool UG>
@@ -689,11 +680,11 @@ extern "C" {
 size_t lgd_gn_act_ws_bytes(const int32_t* level_hw_host, int L, int B, int C, int G, int dtype, int backward) {
     lgd::GaArgs a;
     if (lgd::ga_plan(a, level_hw_host, L, B, C, G, dtype) != LGD_OK) return (size_t)-1;
-    const size_t chunks = lgd::ga_chunks(a);
+    const size_t rows = lgd::ga_rows(a);
     if (lgd::ga_slab_takes(level_hw_host, L, B, C, G, dtype)) return backward && L * B > 1 ? lgd::ga_round((size_t)L * B * C * 2 * sizeof(double)) : 0;
-    if (!backward) return lgd::ga_round(chunks * (size_t)(a.whole ? G : a.P) * 2 * sizeof(double));
-    return lgd::ga_round(chunks * (size_t)(a.whole ? C : a.P) * 2 * sizeof(float)) + lgd::ga_round((size_t)L * B * C * 2 * sizeof(double)) +
-           lgd::ga_round((size_t)L * B * G * 2 * sizeof(float)) + (a.fused ? lgd::ga_round(chunks * (size_t)G * 2 * sizeof(float)) : 0);
+    if (!backward) return lgd::ga_round(rows * G * 2 * sizeof(double));
+    return lgd::ga_round(rows * C * 2 * sizeof(float)) + lgd::ga_round((size_t)L * B * C * 2 * sizeof(double)) +
+           lgd::ga_round((size_t)L * B * G * 2 * sizeof(float)) + (a.fused ? lgd::ga_round(rows * G * 2 * sizeof(float)) : 0);
 }
 
 int lgd_gn_act_fwd(const void* const* x_host, const int32_t* level_hw_host, int L, int B, int C, int G, int dtype, const void* gamma,
@@ -707,7 +698,6 @@ int lgd_gn_act_fwd(const void* const* x_host, const int32_t* level_hw_host, int 
         a.x[l] = x_host[l]; a.out[l] = y_host[l];
     }
     a.gamma = gamma; a.beta = beta; a.ptype = param_dtype; a.eps = eps;
-    a.W = a.whole ? G : a.P;
     a.partd = static_cast<double*>(ws); a.stats = stats;
     hipStream_t s = (hipStream_t)stream;
     const lgd::GaCall c = {x_host, nullptr, y_host, level_hw_host, L, B, C, G, dtype, act, param_dtype, eps, gamma, beta, stats, nullptr, nullptr, nullptr};
@@ -740,10 +730,9 @@ int lgd_gn_act_bwd(const void* const* x_host, const void* const* dy_host, const 
             LGD_LAUNCH("gn_act_bwd_param_kernel", lgd::ga_param_kernel, dim3((unsigned)((C + 63) / 64)), dim3(256), 0, s, a);
         return lgd::check_launch();
     }
-    a.W = a.whole ? C : a.P;
     w += lgd::ga_round((size_t)L * B * C * 2 * sizeof(double));
     a.partf = reinterpret_cast<float*>(w);
-    w += lgd::ga_round(lgd::ga_chunks(a) * (size_t)a.W * 2 * sizeof(float));
+    w += lgd::ga_round(lgd::ga_rows(a) * (size_t)C * 2 * sizeof(float));
     a.bstats = reinterpret_cast<float*>(w);
     w += lgd::ga_round((size_t)L * B * G * 2 * sizeof(float));
     a.partg = reinterpret_cast<float*>(w);

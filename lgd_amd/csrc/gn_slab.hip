@@ -192,7 +192,7 @@ __global__ __launch_bounds__(kSlabThreads) void slab_fwd_kernel(SlabArgs a) {
         if (u >= mine) continue;
         float z[E];
         #pragma unroll
-        for (int i = 0; i < E; ++i) z[i] = (float)fma((double)slab_get<T>(x[u].w, i), A[i], Bc[i]);
+        for (int i = 0; i < E; ++i) z[i] = ga_single(fma((double)slab_get<T>(x[u].w, i), A[i], Bc[i]));
         if (a.act == kActRelu) {
             #pragma unroll
             for (int i = 0; i < E; ++i) z[i] = ga_act<kActRelu>(z[i]);

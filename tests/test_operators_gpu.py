@@ -105,6 +105,10 @@ GN_SHAPES = [
     (2, 2056, 8, [(3, 5)]),                          # 257 (514) vectors a row: column blocks
     (1, 1025, 5, [(4, 3)]),                          # odd and wide: column blocks over wrapped rows
     (2, 1026, 1026, [(2, 3)]),                       # as many groups as channels, over column blocks
+    (2, 2600, 8, [(9, 11)]),                         # column blocks that cut groups (fp32) or hold them whole
+    (1, 2048, 32, [(23, 19)]), (2, 4096, 64, [(21, 22)]),   # column blocks of whole groups (fp32; all types)
+    (3, 517, 11, [(20, 21)]),                        # an odd row over two column blocks: every block has all channels
+    (2, 1280, 32, [(30, 31)]), (2, 660, 4, [(37, 31)]),   # 160 and 165 vectors a row: 320 and 192 threads
     (1, 256, 32, [(40, 67)]),                        # more than one chunk a sample
     (5, 96, 1, [(17, 19), (2, 2)]),                  # one group
 ]
