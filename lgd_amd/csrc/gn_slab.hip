@@ -355,7 +355,7 @@ static bool slab_plan(SlabArgs& a, SlabPlan& p, const GaCall& c) {
     long long total = 0;
     for (int l = 0; l < c.L; ++l) total += (long long)c.hw[2 * l] * c.hw[2 * l + 1] * c.B * c.C;
     const long long slab = (long long)most * ng * cg, cu = slab > total / 256 ? slab : total / 256;
-    if (cu > 24576LL * (row < 16 ? row : 16) / 16 / (p.VW == 1 ? 2 : 1)) return false;
+    if (cu > 24576LL * (row < 16 ? row : 16) / 16 / (p.VW == 1 ? 2 : 1) / (ng > 1 ? 2 : 1)) return false;   // (several groups: 16 K 16 / 11)
     a = SlabArgs{};
     a.VR = row / (4 * p.VW);
     if (a.VR > kSlabThreads || ng * cg > kSlabCh || (long long)most * c.C * size >= (1LL << 32)) return false;   // (32-bit offsets in a sample)

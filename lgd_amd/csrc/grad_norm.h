@@ -34,11 +34,11 @@ template <typename T> __device__ __forceinline__ int norm_head(const T* p, int c
     return h < count ? h : count;
 }
 
-// `count` contiguous elements by a workgroup of 256 threads: 16-byte loads between an unaligned head and tail, U of them in flight
+// `count` contiguous elements by 256 threads (t: 0 .. 255): 16-byte loads between an unaligned head and tail, U of them in flight
 template <int NT, typename T, int U, bool STREAM>
-__device__ __forceinline__ void norm_chunk(const T* __restrict__ p, int count, NormAcc<NT>& acc) {
+__device__ __forceinline__ void norm_chunk(const T* __restrict__ p, int count, NormAcc<NT>& acc, int t) {
     constexpr int V = Vec16<T>::V;
-    const int t = threadIdx.x, head = norm_head(p, count), nv = (count - head) / V, tail = head + nv * V;
+    const int head = norm_head(p, count), nv = (count - head) / V, tail = head + nv * V;
     const T* q = p + head;
     for (int i0 = t; i0 < nv; i0 += 256 * U) {
         lgd_u32x4 v[U];
@@ -80,15 +80,15 @@ struct TensorFinder {
 };
 template <int K, typename First> __device__ __forceinline__ TensorFinder<K, First> tensor_finder(First f, int lo, int hi) { return TensorFinder<K, First>(f, lo, hi); }
 
-// the workgroup's accumulators as one, in every thread (sh: 4 words; barriers inside)
-template <int NT>
+// the workgroup's accumulators as one, in every thread (sh: a word per wave; barriers inside)
+template <int NT, int WAVES = 4>
 __device__ __forceinline__ NormAcc<NT> norm_block(NormAcc<NT> acc, double* sh) {
     acc.wave();
     __syncthreads();
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = acc.word();
     __syncthreads();
     acc = NormAcc<NT>::from(sh[0]);
-    for (int i = 1; i < 4; ++i) acc.join(NormAcc<NT>::from(sh[i]));
+    for (int i = 1; i < WAVES; ++i) acc.join(NormAcc<NT>::from(sh[i]));
     return acc;
 }
 

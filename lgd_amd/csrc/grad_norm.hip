@@ -16,6 +16,8 @@ constexpr int kNormGrid = 1024;      // workgroups at most: 4 per CU
 constexpr int kNormUnroll = 4;       // 16-byte accesses of a thread in flight
 constexpr int kNormInline = 160;     // records in the kernel arguments (24 bytes each, under 4 KB)
 
+constexpr int kNormOnce = 8;         // chunks of a list that one workgroup takes alone: 3.7 us against 4.3 at 8 tensors of 1000, 5.4 against 4.3 at 16
+
 struct NormEntry {
     void* p;
     long long n;
@@ -46,14 +48,17 @@ __global__ __launch_bounds__(256) void norm_table_kernel(NormTable t, NormEntry*
 }
 
 template <int NT, bool STREAM>
+__device__ __forceinline__ void norm_entry(const NormEntry& e, long long first, int count, NormAcc<NT>& acc, int t) {
+    if (e.dtype == LGD_F32) norm_chunk<NT, float, kNormUnroll, STREAM>(static_cast<const float*>(e.p) + first, count, acc, t);
+    else if (e.dtype == LGD_BF16) norm_chunk<NT, __bf16, kNormUnroll, STREAM>(static_cast<const __bf16*>(e.p) + first, count, acc, t);
+    else norm_chunk<NT, _Float16, kNormUnroll, STREAM>(static_cast<const _Float16*>(e.p) + first, count, acc, t);
+}
+
+template <int NT, bool STREAM>
 __global__ __launch_bounds__(256) void norm_partial_kernel(NormTable t, double* part) {
     __shared__ double sh[4];
     NormAcc<NT> acc;
-    norm_walk(t, blockIdx.x, gridDim.x, [&](const NormEntry& e, long long first, int count) {
-        if (e.dtype == LGD_F32) norm_chunk<NT, float, kNormUnroll, STREAM>(static_cast<const float*>(e.p) + first, count, acc);
-        else if (e.dtype == LGD_BF16) norm_chunk<NT, __bf16, kNormUnroll, STREAM>(static_cast<const __bf16*>(e.p) + first, count, acc);
-        else norm_chunk<NT, _Float16, kNormUnroll, STREAM>(static_cast<const _Float16*>(e.p) + first, count, acc);
-    });
+    norm_walk(t, blockIdx.x, gridDim.x, [&](const NormEntry& e, long long first, int count) { norm_entry<NT, STREAM>(e, first, count, acc, threadIdx.x); });
     acc = norm_block<NT>(acc, sh);
     if (threadIdx.x == 0) part[blockIdx.x] = acc.word();
 }
@@ -66,9 +71,9 @@ __global__ __launch_bounds__(256) void norm_final_kernel(const double* part, int
 }
 
 template <typename T, int U>
-__device__ __forceinline__ void norm_scale_chunk(T* p, int count, float c) {
+__device__ __forceinline__ void norm_scale_chunk(T* p, int count, float c, int t) {
     constexpr int V = Vec16<T>::V;
-    const int t = threadIdx.x, head = norm_head(p, count), nv = (count - head) / V, tail = head + nv * V;
+    const int head = norm_head(p, count), nv = (count - head) / V, tail = head + nv * V;
     T* q = p + head;
     for (int i0 = t; i0 < nv; i0 += 256 * U) {
         lgd_u32x4 v[U];
@@ -88,17 +93,34 @@ __device__ __forceinline__ void norm_scale_chunk(T* p, int count, float c) {
     if (t < count - tail) glob_store(p + tail + t, (T)((float)glob_load(p + tail + t) * c));
 }
 
+__device__ __forceinline__ void scale_entry(const NormEntry& e, long long first, int count, float c, int t) {
+    if (e.dtype == LGD_F32) norm_scale_chunk<float, kNormUnroll>(static_cast<float*>(e.p) + first, count, c, t);
+    else if (e.dtype == LGD_BF16) norm_scale_chunk<__bf16, kNormUnroll>(static_cast<__bf16*>(e.p) + first, count, c, t);
+    else norm_scale_chunk<_Float16, kNormUnroll>(static_cast<_Float16*>(e.p) + first, count, c, t);
+}
+
 template <int NT>
 __global__ __launch_bounds__(256) void norm_scale_kernel(NormTable t, const double* part, int np, float max_norm, float* out) {
     __shared__ double sh[4];
     const float norm = norm_total<NT>(part, np, sh), c = norm_coef(norm, max_norm);
     if (blockIdx.x == 0 && threadIdx.x == 0) *out = norm;
     if (c == 1.f) return;
-    norm_walk(t, blockIdx.x, gridDim.x, [&](const NormEntry& e, long long first, int count) {
-        if (e.dtype == LGD_F32) norm_scale_chunk<float, kNormUnroll>(static_cast<float*>(e.p) + first, count, c);
-        else if (e.dtype == LGD_BF16) norm_scale_chunk<__bf16, kNormUnroll>(static_cast<__bf16*>(e.p) + first, count, c);
-        else norm_scale_chunk<_Float16, kNormUnroll>(static_cast<_Float16*>(e.p) + first, count, c);
-    });
+    norm_walk(t, blockIdx.x, gridDim.x, [&](const NormEntry& e, long long first, int count) { scale_entry(e, first, count, c, threadIdx.x); });
+}
+
+// a list of at most kNormOnce chunks: everything in one workgroup of four teams of 256, one launch
+template <int NT, bool CLIP>
+__global__ __launch_bounds__(1024) void norm_once_kernel(NormTable t, float max_norm, float* out) {
+    __shared__ double sh[16];
+    const int team = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8), tid = threadIdx.x & 255;
+    NormAcc<NT> acc;
+    norm_walk(t, team, 4, [&](const NormEntry& e, long long first, int count) { norm_entry<NT, false>(e, first, count, acc, tid); });
+    const float norm = norm_block<NT, 16>(acc, sh).value();
+    if (threadIdx.x == 0) *out = norm;
+    if (!CLIP) return;
+    const float c = norm_coef(norm, max_norm);
+    if (c == 1.f) return;
+    norm_walk(t, team, 4, [&](const NormEntry& e, long long first, int count) { scale_entry(e, first, count, c, tid); });
 }
 
 static size_t norm_ws_part() { return (size_t)kNormGrid * sizeof(double); }
@@ -137,6 +159,11 @@ static int norm_table(NormTable& t, const lgd_grad_tensor* host, int n, void* ws
 template <int NT>
 static int norm_run(const NormTable& t, int grid, bool clip, float max_norm, void* ws, float* out, hipStream_t s) {
     double* part = static_cast<double*>(ws);
+    if (t.nblk <= kNormOnce && !t.more) {
+        if (clip) LGD_LAUNCH("grad_clip_kernel", (norm_once_kernel<NT, true>), dim3(1), dim3(1024), 0, s, t, max_norm, out);
+        else LGD_LAUNCH("grad_norm_kernel", (norm_once_kernel<NT, false>), dim3(1), dim3(1024), 0, s, t, max_norm, out);
+        return check_launch();
+    }
     if (clip) LGD_LAUNCH("grad_norm_kernel", (norm_partial_kernel<NT, false>), dim3((unsigned)grid), dim3(256), 0, s, t, part);
     else LGD_LAUNCH("grad_norm_kernel", (norm_partial_kernel<NT, true>), dim3((unsigned)grid), dim3(256), 0, s, t, part);
     if (clip) LGD_LAUNCH("grad_clip_kernel", norm_scale_kernel<NT>, dim3((unsigned)grid), dim3(256), 0, s, t, part, grid, max_norm, out);

@@ -159,7 +159,7 @@ __global__ __launch_bounds__(256) void sgd_norm_kernel(const lgd_sgd_tensor* __r
     for (int c = g.blk[k] + (int)blockIdx.x; c < g.blk[k + 1]; c += kSgdNormGrid) {
         const int i = finder.find(c);
         const long long first = (long long)(c - blk_off[i]) * kSgdChunk, left = tab[i].n - first;
-        norm_chunk<NT, float, 4, false>(tab[i].g + first, (int)(left < kSgdChunk ? left : kSgdChunk), acc);
+        norm_chunk<NT, float, 4, false>(tab[i].g + first, (int)(left < kSgdChunk ? left : kSgdChunk), acc, threadIdx.x);
     }
     acc = norm_block<NT>(acc, sh);
     if (threadIdx.x == 0) part[k * kSgdNormGrid + blockIdx.x] = acc.word();
