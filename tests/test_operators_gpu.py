@@ -126,6 +126,23 @@ def test_group_norm_act(shape, act, dtype):
     _check(xs, G, w, b, act, 1e-5, dys, ys, dxs, dw, db)
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape", [(1, 1040, 520, [(80, 81)]), (1, 96, 48, [(150, 203)]), (2, 1040, 520, [(9, 11), (120, 61)]), (1, 1025, 205, [(67, 66)])], ids=str)
+def test_group_norm_act_many_groups(shape, dtype):
+    """more groups and chunks than the apply kernels reduce themselves: the records go through kernels of their own; parameters frozen, too"""
+    B, C, G, hws = shape
+    T = TYPES[dtype]
+    xs, dys = _maps(B, C, hws, T, 400, 0.7, -0.3), _maps(B, C, hws, T, 500)
+    w, b = _params(C, torch.float32, 600)
+    ys, dxs, dw, db = _run(xs, G, w, b, "silu", 1e-5, dys)
+    _check(xs, G, w, b, "silu", 1e-5, dys, ys, dxs, dw, db)
+    yf, df, _, _ = _run(xs, G, None, None, "relu", 1e-5, dys)
+    _check(xs, G, None, None, "relu", 1e-5, dys, yf, df, None, None)
+    from lgd_amd import ops
+    gw, gb = torch.autograd.grad(ops.group_norm_act(xs, G, w, b, act="silu"), [w, b], dys)   # maps without gradients
+    assert torch.equal(gw, dw) and torch.equal(gb, db)
+
+
 @pytest.mark.parametrize("weight,bias,ptype", [(True, False, "fp32"), (False, True, "bf16"), (False, False, "fp32"), (True, True, "fp16"), (True, True, "fp32")])
 def test_group_norm_act_parameters(weight, bias, ptype):
     """either parameter may be missing, and theirs may be another type than the maps'"""
