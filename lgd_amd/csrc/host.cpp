@@ -1,12 +1,14 @@
-// Host side of the operators whose calls are short beside their Python: group_norm_act (its checks, allocations and autograd node) and the gradient
-// lists of grad_norm / clip_grad_norm_ (one pass over the tensors).  A CPython extension over torch's C++ API; everything that runs on the GPU goes
-// through the C ABI of include/lgd_hip.h, whose entry points lgd_amd/hip.py hands over (bind), so that both see the same library.
+// Host side of the operators whose calls are short beside their Python: group_norm_act (its checks, allocations and autograd node), the gradient
+// lists of grad_norm / clip_grad_norm_ (one pass over the tensors) and the table of the fused SGD step.  A CPython extension over torch's C++ API;
+// everything that runs on the GPU goes through the C ABI of include/lgd_hip.h, whose entry points lgd_amd/hip.py hands over (bind), so that both see
+// the same library.
 // What it is for: a training call on small maps costs the host two autograd.Function halves on two threads, 145 us on the MI355X host where the GPU needs
-// 25; a list of 160 gradients 62 us for 16.
+// 25; a list of 160 gradients 62 us for 16; the step over 10 (160) tensors 37 (60) us in Python, 17 (27) here.
 #include <Python.h>
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
@@ -34,6 +36,9 @@ struct {
     decltype(&lgd_grad_norm_ws_bytes) norm_ws;
     decltype(&lgd_grad_norm) norm;
     decltype(&lgd_grad_clip) clip;
+    decltype(&lgd_sgd_clip_step) sgd_clip;
+    decltype(&lgd_sgd_norm_ws_bytes) sgd_norm_ws;
+    decltype(&lgd_sgd_norm_step) sgd_norm;
     decltype(&lgd_last_error) last_error;
     PyObject* error = nullptr;   // LgdHipError
 } api;
@@ -258,9 +263,16 @@ std::vector<Tensor> tensors_of(PyObject* seq, bool grads) {
     return out;
 }
 
+using Runs = std::vector<std::pair<uintptr_t, uintptr_t>>;   // addresses: first, behind the last
+void refuse_overlap(Runs& runs) {
+    std::sort(runs.begin(), runs.end());
+    for (size_t i = 1; i < runs.size(); ++i)
+        if (runs[i - 1].second > runs[i].first) refuse("two of the gradients share memory: each element can be clipped once");
+}
+
 // in-place scaling needs every element once: a gradient listed twice, an expanded one, or views that overlap are refused
 void refuse_shared(const std::vector<Tensor>& ts, const std::vector<Tensor>& flat) {
-    std::vector<std::pair<uintptr_t, uintptr_t>> runs;
+    Runs runs;
     std::vector<const void*> strided;
     for (size_t i = 0; i < ts.size(); ++i) {
         if (ts[i].numel() == 0) continue;
@@ -271,9 +283,7 @@ void refuse_shared(const std::vector<Tensor>& ts, const std::vector<Tensor>& fla
         for (int64_t d = 0; d < ts[i].dim(); ++d)
             if (ts[i].stride(d) == 0 && ts[i].size(d) > 1) refuse("a gradient that is expanded, or listed twice, cannot be clipped in place");
     }
-    std::sort(runs.begin(), runs.end());
-    for (size_t i = 1; i < runs.size(); ++i)
-        if (runs[i - 1].second > runs[i].first) refuse("two of the gradients share memory: each element can be clipped once");
+    refuse_overlap(runs);
     std::sort(strided.begin(), strided.end());
     if (std::adjacent_find(strided.begin(), strided.end()) != strided.end()) refuse("a gradient that is expanded, or listed twice, cannot be clipped in place");
 }
@@ -308,13 +318,85 @@ Tensor norm_of(const std::vector<Tensor>& ts, int norm_type, bool clip, double m
     return out;
 }
 
+// ------------------------------------------------------------------------------------------- the fused step
+bool dense_f32(const Tensor& t) { return t.layout() == at::kStrided && t.scalar_type() == at::kFloat && t.is_contiguous(); }
+
+// what follows from the set of parameters that have a gradient, laid out by lgd_amd/optim.py
+struct SgdPlan {
+    const int32_t* rows;           // the parameters of the table's rows, ascending
+    const lgd_sgd_tensor* table;   // n and reserved filled in
+    const int32_t* blk;            // [k + 1]
+    const int32_t* set;            // [k] which hyper-parameters
+    const int32_t* border;         // [groups + 1] rows and blocks of the optimizers
+    const int32_t* border_blk;
+    int k, groups;
+};
+enum class Sgd { kDone, kOtherSet, kNotGpu };
+
+Sgd sgd_step(PyObject* params, PyObject* momenta, const SgdPlan& plan, const std::vector<float>& hyper, bool by_norm, int norm_type, double clip, Tensor& norms) {
+    const int n = (int)PyList_GET_SIZE(params), k = plan.k;
+    std::vector<Tensor> ps, gs, ms;
+    ps.reserve(k); gs.reserve(k); ms.reserve(k);
+    for (int i = 0, j = 0; i < n; ++i) {
+        const Tensor& p = THPVariable_Unpack(PyList_GET_ITEM(params, i));
+        const Tensor& g = p.grad();
+        const bool row = j < k && plan.rows[j] == i;
+        if (g.defined() != row) return Sgd::kOtherSet;
+        if (!row) continue;
+        ps.push_back(p); gs.push_back(g); ms.push_back(THPVariable_Unpack(PyList_GET_ITEM(momenta, i)));
+        ++j;
+    }
+    const c10::Device dev = gs[0].device();
+    if (!dev.is_cuda()) return Sgd::kNotGpu;
+    const c10::DeviceGuard guard(dev);
+    if (by_norm && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
+        refuse("the fused step uploads its table from host memory that later steps reuse: it cannot be captured into a graph");
+    at::AutoDispatchBelowADInplaceOrView below;
+    const int64_t bytes = (int64_t)k * sizeof(lgd_sgd_tensor) + 4 * (k + 1), room = (bytes + 15) / 16 * 16;
+    // torch hands a pinned block out again only after the copies that read it
+    const Tensor host = at::empty({bytes}, at::TensorOptions().dtype(at::kByte).pinned_memory(true));
+    lgd_sgd_tensor* t = static_cast<lgd_sgd_tensor*>(host.data_ptr());
+    memcpy(t, plan.table, (size_t)k * sizeof(lgd_sgd_tensor));
+    memcpy(t + k, plan.blk, 4 * (size_t)(k + 1));
+    Runs runs;
+    for (int j = 0; j < k; ++j) {
+        if (!dense_f32(gs[j]) || gs[j].device() != dev) refuse("fused SGD needs dense contiguous fp32 gradients on one device");
+        if (!dense_f32(ps[j])) refuse("fused SGD needs dense contiguous fp32 parameters");
+        t[j].p = ps[j].data_ptr<float>(); t[j].g = gs[j].data_ptr<float>(); t[j].m = ms[j].data_ptr<float>();
+        const float* h = &hyper[3 * (size_t)plan.set[j]];
+        t[j].lr = h[0]; t[j].wd = h[1]; t[j].mu = h[2];
+        if (by_norm && t[j].n > 0) runs.emplace_back((uintptr_t)t[j].g, (uintptr_t)(t[j].g + t[j].n));
+    }
+    refuse_overlap(runs);
+    const int64_t ws = by_norm ? (int64_t)api.sgd_norm_ws(plan.groups) : 0;
+    Tensor work = at::empty({room + ws}, at::TensorOptions().device(dev).dtype(at::kByte));
+    work.narrow(0, 0, bytes).copy_(host, true);
+    char* base = static_cast<char*>(work.data_ptr());
+    const auto* table = reinterpret_cast<const lgd_sgd_tensor*>(base);
+    const auto* blk = reinterpret_cast<const int32_t*>(table + k);
+    void* stream = stream_of(work);
+    if (by_norm) {
+        norms = at::empty({plan.groups}, at::TensorOptions().device(dev).dtype(at::kFloat));
+        check(api.sgd_norm(table, blk, k, plan.blk[k], plan.border, plan.border_blk, plan.groups, norm_type, (float)clip, base + room, norms.data_ptr<float>(), stream), "lgd_sgd_norm_step");
+    } else {
+        check(api.sgd_clip(table, blk, k, plan.blk[k], (float)clip, stream), "lgd_sgd_clip_step");
+    }
+    // written through raw pointers: autograd's version counters, which the fold caches (ConvBN._frozen_fold, FrozenBatchNorm2d.scale_shift) key on and the
+    // saved-tensor check reads
+    for (int j = 0; j < k; ++j) {
+        torch::autograd::impl::bump_version(ps[j]); torch::autograd::impl::bump_version(gs[j]); torch::autograd::impl::bump_version(ms[j]);
+    }
+    return Sgd::kDone;
+}
+
 // ------------------------------------------------------------------------------------------- Python
 // bind(error class, address of every entry point in the order of `api`)
 PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 8) { PyErr_SetString(PyExc_TypeError, "bind(error, 7 addresses)"); return nullptr; }
-    void* p[7];
-    for (int i = 0; i < 7; ++i) {
+    constexpr int kEntries = 10;
+    if (n != 1 + kEntries) { PyErr_SetString(PyExc_TypeError, "bind(error, addresses of the entry points)"); return nullptr; }
+    void* p[kEntries];
+    for (int i = 0; i < kEntries; ++i) {
         p[i] = PyLong_AsVoidPtr(a[i + 1]);
         if (!p[i]) { if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "null entry point"); return nullptr; }
     }
@@ -323,7 +405,8 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
     api.error = a[0];
     api.gn_ws = (decltype(api.gn_ws))p[0]; api.gn_fwd = (decltype(api.gn_fwd))p[1]; api.gn_bwd = (decltype(api.gn_bwd))p[2];
     api.norm_ws = (decltype(api.norm_ws))p[3]; api.norm = (decltype(api.norm))p[4]; api.clip = (decltype(api.clip))p[5];
-    api.last_error = (decltype(api.last_error))p[6];
+    api.sgd_clip = (decltype(api.sgd_clip))p[6]; api.sgd_norm_ws = (decltype(api.sgd_norm_ws))p[7]; api.sgd_norm = (decltype(api.sgd_norm))p[8];
+    api.last_error = (decltype(api.last_error))p[9];
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }
@@ -398,9 +481,58 @@ PyObject* py_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// sgd_step(parameters, momentum buffers, plan, [lr, weight decay, momentum] of every set, norm code or None, clip) -> the norms (by value: True);
+// None: the parameters that have a gradient are not the plan's; False: they are not on a GPU.  Lists of tensors (None where a parameter has no row);
+// plan: six bytes objects in the order of SgdPlan
+PyObject* py_sgd_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 6 || !PyList_Check(a[0]) || !PyList_Check(a[1]) || PyList_GET_SIZE(a[0]) != PyList_GET_SIZE(a[1]) || !PyTuple_Check(a[2]) || PyTuple_GET_SIZE(a[2]) != 6 || !PyList_Check(a[3])) {
+        PyErr_SetString(PyExc_TypeError, "sgd_step(list, list, plan, list, norm code, clip)");
+        return nullptr;
+    }
+    const void* part[6];
+    Py_ssize_t size[6];
+    for (int i = 0; i < 6; ++i) {
+        PyObject* b = PyTuple_GET_ITEM(a[2], i);
+        if (!PyBytes_Check(b)) { PyErr_SetString(PyExc_TypeError, "a plan holds bytes"); return nullptr; }
+        part[i] = PyBytes_AS_STRING(b); size[i] = PyBytes_GET_SIZE(b);
+    }
+    SgdPlan plan = {static_cast<const int32_t*>(part[0]), static_cast<const lgd_sgd_tensor*>(part[1]), static_cast<const int32_t*>(part[2]), static_cast<const int32_t*>(part[3]),
+                    static_cast<const int32_t*>(part[4]), static_cast<const int32_t*>(part[5]), (int)(size[0] / 4), (int)(size[4] / 4) - 1};
+    std::vector<float> hyper;
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(a[3]); ++i) hyper.push_back((float)PyFloat_AsDouble(PyList_GET_ITEM(a[3], i)));
+    const bool by_norm = a[4] != Py_None;
+    const long code = by_norm ? PyLong_AsLong(a[4]) : 0;
+    const double clip = PyFloat_AsDouble(a[5]);
+    if (PyErr_Occurred()) return nullptr;
+    bool fits = plan.k > 0 && size[1] == (Py_ssize_t)(plan.k * sizeof(lgd_sgd_tensor)) && size[2] == 4 * (plan.k + 1) && size[3] == 4 * plan.k && plan.groups > 0 && size[5] == size[4];
+    for (Py_ssize_t i = 0; fits && i < PyList_GET_SIZE(a[0]); ++i) fits = THPVariable_Check(PyList_GET_ITEM(a[0], i));
+    for (int j = 0; fits && j < plan.k; ++j) {
+        const Py_ssize_t i = plan.rows[j];
+        fits = i >= 0 && i < PyList_GET_SIZE(a[0]) && THPVariable_Check(PyList_GET_ITEM(a[1], i)) && plan.set[j] >= 0 && 3 * (size_t)plan.set[j] + 3 <= hyper.size() &&
+               plan.table[j].n == THPVariable_Unpack(PyList_GET_ITEM(a[0], i)).numel() && plan.table[j].n == THPVariable_Unpack(PyList_GET_ITEM(a[1], i)).numel();
+    }
+    if (!fits) { PyErr_SetString(PyExc_ValueError, "the plan does not fit the lists"); return nullptr; }
+    try {
+        Tensor norms;
+        switch (sgd_step(a[0], a[1], plan, hyper, by_norm, (int)code, clip, norms)) {
+            case Sgd::kOtherSet: Py_RETURN_NONE;
+            case Sgd::kNotGpu: Py_RETURN_FALSE;
+            default: break;
+        }
+        if (!by_norm) Py_RETURN_TRUE;
+        return THPVariable_Wrap(norms);
+    } catch (const Refused& e) {
+        PyErr_SetString(api.error, e.what());
+        return nullptr;
+    }
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {{"bind", (PyCFunction)(void (*)())py_bind, METH_FASTCALL, nullptr},
                          {"group_norm_act", (PyCFunction)(void (*)())py_group_norm_act, METH_FASTCALL, nullptr},
                          {"norm", (PyCFunction)(void (*)())py_norm, METH_FASTCALL, nullptr},
+                         {"sgd_step", (PyCFunction)(void (*)())py_sgd_step, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_lgd_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -187,7 +187,8 @@ def load():
 
 
 _HOST_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "_lgd_host.so")
-_HOST_ENTRIES = ("lgd_gn_act_ws_bytes", "lgd_gn_act_fwd", "lgd_gn_act_bwd", "lgd_grad_norm_ws_bytes", "lgd_grad_norm", "lgd_grad_clip", "lgd_last_error")
+_HOST_ENTRIES = ("lgd_gn_act_ws_bytes", "lgd_gn_act_fwd", "lgd_gn_act_bwd", "lgd_grad_norm_ws_bytes", "lgd_grad_norm", "lgd_grad_clip",
+                 "lgd_sgd_clip_step", "lgd_sgd_norm_ws_bytes", "lgd_sgd_norm_step", "lgd_last_error")
 _host = None
 
 

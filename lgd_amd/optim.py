@@ -10,8 +10,6 @@ schedulers drive their `lr`), so checkpoints and `Trainer.state_dict()` are unch
 ops and two optimizers) and ~40 launches over 13 tensor transfers per element; at 2 images per GPU the GPU ran dry for 0.7 ms at the
 optimizer entry.  Here the host builds one table (three pointers, length, lr / wd / mu per tensor) in pinned memory and launches once.
 """
-import ctypes
-
 import numpy as np
 import torch
 
@@ -85,7 +83,6 @@ class FusedClipSGD:
     clip_value: element-wise clamp.  clip_norm: the gradients of EACH optimizer are scaled by min(1, clip_norm / (norm + 1e-6)) of their own
     norm (norm_type 2, 1 or inf) -- torch.nn.utils.clip_grad_norm_ per optimizer, then its step(); `total_norms` then holds the norms
     before clipping of the last step (one fp32 per optimizer, on the device).  Neither: no clipping.  The clipped gradients are written back."""
-    SLOTS = 8  # pinned staging tables in flight (a slot is reused SLOTS steps later, after its upload event has completed)
 
     def __init__(self, optimizers, clip_value=None, clip_norm=None, norm_type=2.0):
         self.optimizers = list(optimizers)
@@ -105,17 +102,10 @@ class FusedClipSGD:
             if len({id(p) for p in self.params}) != n or not 1 <= len(self.optimizers) <= 16:
                 raise hip.LgdHipError("clipping by norm takes 1 to 16 optimizers (LGD_MAX_SGD_GROUPS) that share no parameter")
         self._numel = np.array([p.numel() for p in self.params], dtype=np.int64)
-        self._m_ptr = np.zeros(n, dtype=np.uint64)
-        self._m_ref = [None] * n   # the buffer each cached pointer belongs to
+        self._m_ref = [None] * n   # momentum buffers
         self._state_ids = None     # Optimizer.load_state_dict installs a new state dict: the cached buffers are then stale
         self._grp = np.array([k * 4096 + gi for k, gi in self.owner], dtype=np.int64)
-        self.chunk = None
-        self._checked_idx = self._plan = None
-        rec = 48 * n + 4 * (n + 1)
-        self._slot_bytes = (rec + 255) // 256 * 256
-        self._pinned = None
-        self._events = [None] * self.SLOTS
-        self._slot = 0
+        self._plan = None
 
     def zero_grad(self):
         """`optimizer.zero_grad(set_to_none=True)` of all the optimizers (plain loop: no per-optimizer bookkeeping)."""
@@ -140,87 +130,52 @@ class FusedClipSGD:
             if not (m.is_cuda and m.dtype == torch.float32 and m.is_contiguous() and m.numel() == p.numel()):
                 raise hip.LgdHipError("momentum buffer of a fused-SGD parameter must be a dense fp32 device tensor")
             self._m_ref[i] = m
-            self._m_ptr[i] = m.data_ptr()
+
+    def _make_plan(self):
+        """(parameter groups whose hyper-parameters the table needs, the columns of csrc/host.cpp's SgdPlan): what follows from the set of
+        parameters that have a gradient; None where none has"""
+        idx = [i for i, p in enumerate(self.params) if p.grad is not None]
+        if not idx:
+            return None
+        hip.require_gpu(self.params[idx[0]].grad)
+        self._buffers(idx)
+        chunk = int(hip.load().lgd_sgd_chunk_elems())
+        ii = np.asarray(idx, dtype=np.int64)
+        tab, blk = np.zeros(len(idx), dtype=_TENSOR_DT), np.zeros(len(idx) + 1, dtype=np.int32)
+        tab["n"] = self._numel[ii]
+        blk[1:] = np.cumsum((self._numel[ii] + chunk - 1) // chunk)
+        keys, which = np.unique(self._grp[ii], return_inverse=True)
+        tab["reserved"] = owner = self._grp[ii] // 4096   # clipping by norm: the row's optimizer
+        border = np.searchsorted(owner, np.arange(len(self.optimizers) + 1))   # the table is ordered by optimizer
+        columns = (ii.astype(np.int32), tab, blk, which.astype(np.int32), border.astype(np.int32), blk[border])
+        return [divmod(key, 4096) for key in keys.tolist()], tuple(c.tobytes() for c in columns)
 
     @torch.no_grad()
     def step(self):
-        lib = hip.load()
-        if self.chunk is None:
-            self.chunk = int(lib.lgd_sgd_chunk_elems())
-        grads = [p.grad for p in self.params]
-        idx = [i for i, g in enumerate(grads) if g is not None]
         by_norm = self.clip_norm is not None
         if by_norm and not float(self.clip_norm) >= 0:
             raise hip.LgdHipError("clip_norm must not be negative, got %r" % (self.clip_norm,))
-        if not idx:
-            if by_norm:
-                self.total_norms = torch.zeros(len(self.optimizers), device=self.params[0].device if self.params else None)
-            return
-        hip.require_gpu(grads[idx[0]])
-        if by_norm and torch.cuda.is_current_stream_capturing():
-            raise hip.LgdHipError("the fused step uploads its table from host memory that later steps reuse: it cannot be captured into a graph")
-        params = [self.params[i] for i in idx]
-        grads = [grads[i] for i in idx]
-        k = len(idx)
-        if idx != self._checked_idx:   # once per set of parameters that receive gradients: layout checks (autograd hands out the same kind of
-            for g in grads:            # tensor every step) and what the table's other columns follow from
-                if g.dtype != torch.float32 or not g.is_contiguous() or g.is_sparse:
-                    raise hip.LgdHipError("fused SGD needs dense contiguous fp32 gradients")
-            ii = np.asarray(idx, dtype=np.int64)
-            tab, blk = np.zeros(k, dtype=_TENSOR_DT), np.zeros(k + 1, dtype=np.int32)
-            tab["n"] = self._numel[ii]
-            blk[1:] = np.cumsum((self._numel[ii] + self.chunk - 1) // self.chunk)
-            keys, which = np.unique(self._grp[ii], return_inverse=True)
-            owner = self._grp[ii] // 4096
-            if by_norm:
-                tab["reserved"] = owner
-            border = np.searchsorted(owner, np.arange(len(self.optimizers) + 1)).astype(np.int32)   # the table is ordered by optimizer
-            self._plan = (ii, tab, blk, [divmod(key, 4096) for key in keys.tolist()], which, border, blk[border])
-            self._checked_idx = idx
-        elif not all(map(torch.Tensor.is_contiguous, grads)):
-            raise hip.LgdHipError("fused SGD needs dense contiguous fp32 gradients")
-        self._buffers(idx)
-        ii, tab, blk, keys, which, border, border_blk = self._plan
-        ptr_of = torch.Tensor.data_ptr
-        gp = list(map(ptr_of, grads))
-        if by_norm and len(set(gp)) < k and len({q for q, g in zip(gp, grads) if g.numel()}) < sum(g.numel() > 0 for g in grads):
-            raise hip.LgdHipError("two of the gradients share memory: each element can be clipped once")
-        tab["p"] = list(map(ptr_of, params))
-        tab["g"] = gp
-        tab["m"] = self._m_ptr[ii]
-        hy = np.array([[g["lr"], g["weight_decay"], g["momentum"]] for g in (self.optimizers[o].param_groups[j] for o, j in keys)], dtype=np.float32)[which]
-        tab["lr"], tab["wd"], tab["mu"] = hy[:, 0], hy[:, 1], hy[:, 2]
-        device = grads[0].device
-        if self._pinned is None:
-            self._pinned = torch.empty(self.SLOTS * self._slot_bytes, dtype=torch.uint8).pin_memory()
-        s = self._slot
-        self._slot = (s + 1) % self.SLOTS
-        if self._events[s] is not None:
-            self._events[s].synchronize()   # SLOTS steps old: long complete unless the host ran that far ahead
-        nbytes = 48 * k + 4 * (k + 1)
-        host = self._pinned[s * self._slot_bytes:s * self._slot_bytes + nbytes]
-        raw = host.numpy()
-        raw[:48 * k] = tab.view(np.uint8)
-        raw[48 * k:] = blk.view(np.uint8)
-        n_blocks = int(blk[k])
-        dev = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        dev.copy_(host, non_blocking=True)
-        ev = self._events[s]
-        if ev is None:
-            ev = self._events[s] = torch.cuda.Event()
-        ev.record()
-        base = dev.data_ptr()
+        code, clip = (_norm_code(self.norm_type), float(self.clip_norm)) if by_norm else (None, self.clip_value)
+        if self._plan is not None and [id(o.state) for o in self.optimizers] != self._state_ids:
+            self._plan = None
+        got = None
+        while got is None:   # a plan serves until another set of parameters has gradients
+            if self._plan is None:
+                self._plan = self._make_plan()
+                if self._plan is None:
+                    if by_norm:
+                        self.total_norms = torch.zeros(len(self.optimizers), device=self.params[0].device if self.params else None)
+                    return
+            keys, columns = self._plan
+            groups = [self.optimizers[o].param_groups[j] for o, j in keys]
+            hyper = [float(g[name]) for g in groups for name in ("lr", "weight_decay", "momentum")]
+            got = hip.host().sgd_step(self.params, self._m_ref, columns, hyper, code, clip)
+            if got is None:
+                self._plan = None
+        if got is False:
+            hip.require_gpu(*[p.grad for p in self.params if p.grad is not None])
+            raise hip.LgdHipError("gradients are not on a GPU")
         if by_norm:
-            ng = len(self.optimizers)
-            norms = torch.empty(ng, dtype=torch.float32, device=device)
-            ws = torch.empty(lib.lgd_sgd_norm_ws_bytes(ng), dtype=torch.uint8, device=device)
-            hip.check(lib.lgd_sgd_norm_step(base, base + 48 * k, k, n_blocks, border.ctypes.data, border_blk.ctypes.data, ng, _norm_code(self.norm_type),
-                                            float(self.clip_norm), ws.data_ptr(), norms.data_ptr(), hip.stream_ptr()), "lgd_sgd_norm_step")
-            self.total_norms = norms
-        else:
-            hip.check(lib.lgd_sgd_clip_step(base, base + 48 * k, k, n_blocks, self.clip_value, hip.stream_ptr()), "lgd_sgd_clip_step")
-        # the kernel wrote p, g and the momentum buffers through raw pointers: tell autograd's version counters, which the fold
-        # caches (ConvBN._frozen_fold, FrozenBatchNorm2d.scale_shift) key on and the saved-tensor check reads
-        torch.autograd.graph.increment_version(params + grads + [self._m_ref[i] for i in idx])
+            self.total_norms = got
         for o in self.optimizers:
             o._opt_called = True   # what the LR schedulers' "scheduler.step() before optimizer.step()" check looks at
