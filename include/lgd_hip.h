@@ -642,6 +642,11 @@ size_t lgd_sgd_norm_ws_bytes(int n_groups);
 int lgd_sgd_norm_step(const lgd_sgd_tensor* table, const int32_t* blk_off, int n_tensors, int n_blocks, const int32_t* group_off_host,
                       const int32_t* group_blk_host /* blk_off at the group borders, n_groups + 1 entries */, int n_groups, int norm_type,
                       float max_norm, void* ws, float* norms_out, void* stream);
+/* the same with the table and blk_off in HOST memory, for at most LGD_SGD_INLINE tensors: they travel in the kernels' arguments (no upload) and
+ * may be overwritten when the call returns. */
+#define LGD_SGD_INLINE 72
+int lgd_sgd_norm_step_host(const lgd_sgd_tensor* table_host, const int32_t* blk_off_host, int n_tensors, int n_blocks, const int32_t* group_off_host,
+                           const int32_t* group_blk_host, int n_groups, int norm_type, float max_norm, void* ws, float* norms_out, void* stream);
 
 /* ------------------------------------------------------------------ GroupNorm + activation, channels last
  * GroupNorm(G, per-channel affine) then act over L maps stored (B, H_l, W_l, C), one module for all of them; dtype LGD_F32 / LGD_BF16 /

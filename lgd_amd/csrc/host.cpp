@@ -3,7 +3,7 @@
 // everything that runs on the GPU goes through the C ABI of include/lgd_hip.h, whose entry points lgd_amd/hip.py hands over (bind), so that both see
 // the same library.
 // What it is for: a training call on small maps costs the host two autograd.Function halves on two threads, 145 us on the MI355X host where the GPU needs
-// 25; a list of 160 gradients 62 us for 16; the step over 10 (160) tensors 37 (60) us in Python, 17 (27) here.
+// 25; a list of 160 gradients 62 us for 16; the step over 10 (160) tensors 37 (60) us in Python, 12 (26) here.
 #include <Python.h>
 
 #include <ATen/ATen.h>
@@ -39,6 +39,7 @@ struct {
     decltype(&lgd_sgd_clip_step) sgd_clip;
     decltype(&lgd_sgd_norm_ws_bytes) sgd_norm_ws;
     decltype(&lgd_sgd_norm_step) sgd_norm;
+    decltype(&lgd_sgd_norm_step_host) sgd_norm_host;
     decltype(&lgd_last_error) last_error;
     PyObject* error = nullptr;   // LgdHipError
 } api;
@@ -350,14 +351,15 @@ Sgd sgd_step(PyObject* params, PyObject* momenta, const SgdPlan& plan, const std
     if (!dev.is_cuda()) return Sgd::kNotGpu;
     const c10::DeviceGuard guard(dev);
     if (by_norm && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
-        refuse("the fused step uploads its table from host memory that later steps reuse: it cannot be captured into a graph");
+        refuse("the fused step's table (addresses, learning rates) is the host's of this call: it cannot be captured into a graph");
     at::AutoDispatchBelowADInplaceOrView below;
     const int64_t bytes = (int64_t)k * sizeof(lgd_sgd_tensor) + 4 * (k + 1), room = (bytes + 15) / 16 * 16;
+    const bool inl = by_norm && k <= LGD_SGD_INLINE;   // the table in the kernels' arguments: no upload
     // torch hands a pinned block out again only after the copies that read it
-    const Tensor host = at::empty({bytes}, at::TensorOptions().dtype(at::kByte).pinned_memory(true));
-    lgd_sgd_tensor* t = static_cast<lgd_sgd_tensor*>(host.data_ptr());
+    const Tensor host = inl ? Tensor() : at::empty({bytes}, at::TensorOptions().dtype(at::kByte).pinned_memory(true));
+    lgd_sgd_tensor own[LGD_SGD_INLINE];
+    lgd_sgd_tensor* t = inl ? own : static_cast<lgd_sgd_tensor*>(host.data_ptr());
     memcpy(t, plan.table, (size_t)k * sizeof(lgd_sgd_tensor));
-    memcpy(t + k, plan.blk, 4 * (size_t)(k + 1));
     Runs runs;
     for (int j = 0; j < k; ++j) {
         if (!dense_f32(gs[j]) || gs[j].device() != dev) refuse("fused SGD needs dense contiguous fp32 gradients on one device");
@@ -369,15 +371,21 @@ Sgd sgd_step(PyObject* params, PyObject* momenta, const SgdPlan& plan, const std
     }
     refuse_overlap(runs);
     const int64_t ws = by_norm ? (int64_t)api.sgd_norm_ws(plan.groups) : 0;
-    Tensor work = at::empty({room + ws}, at::TensorOptions().device(dev).dtype(at::kByte));
-    work.narrow(0, 0, bytes).copy_(host, true);
+    Tensor work = at::empty({(inl ? 0 : room) + ws}, at::TensorOptions().device(dev).dtype(at::kByte));
     char* base = static_cast<char*>(work.data_ptr());
+    void* stream = stream_of(work);
+    if (!inl) {
+        memcpy(t + k, plan.blk, 4 * (size_t)(k + 1));
+        work.narrow(0, 0, bytes).copy_(host, true);
+    }
     const auto* table = reinterpret_cast<const lgd_sgd_tensor*>(base);
     const auto* blk = reinterpret_cast<const int32_t*>(table + k);
-    void* stream = stream_of(work);
     if (by_norm) {
         norms = at::empty({plan.groups}, at::TensorOptions().device(dev).dtype(at::kFloat));
-        check(api.sgd_norm(table, blk, k, plan.blk[k], plan.border, plan.border_blk, plan.groups, norm_type, (float)clip, base + room, norms.data_ptr<float>(), stream), "lgd_sgd_norm_step");
+        float* out = norms.data_ptr<float>();
+        check(inl ? api.sgd_norm_host(t, plan.blk, k, plan.blk[k], plan.border, plan.border_blk, plan.groups, norm_type, (float)clip, base, out, stream)
+                  : api.sgd_norm(table, blk, k, plan.blk[k], plan.border, plan.border_blk, plan.groups, norm_type, (float)clip, base + room, out, stream),
+              "lgd_sgd_norm_step");
     } else {
         check(api.sgd_clip(table, blk, k, plan.blk[k], (float)clip, stream), "lgd_sgd_clip_step");
     }
@@ -393,7 +401,7 @@ Sgd sgd_step(PyObject* params, PyObject* momenta, const SgdPlan& plan, const std
 // bind(error class, address of every entry point in the order of `api`)
 PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    constexpr int kEntries = 10;
+    constexpr int kEntries = 11;
     if (n != 1 + kEntries) { PyErr_SetString(PyExc_TypeError, "bind(error, addresses of the entry points)"); return nullptr; }
     void* p[kEntries];
     for (int i = 0; i < kEntries; ++i) {
@@ -406,7 +414,7 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
     api.gn_ws = (decltype(api.gn_ws))p[0]; api.gn_fwd = (decltype(api.gn_fwd))p[1]; api.gn_bwd = (decltype(api.gn_bwd))p[2];
     api.norm_ws = (decltype(api.norm_ws))p[3]; api.norm = (decltype(api.norm))p[4]; api.clip = (decltype(api.clip))p[5];
     api.sgd_clip = (decltype(api.sgd_clip))p[6]; api.sgd_norm_ws = (decltype(api.sgd_norm_ws))p[7]; api.sgd_norm = (decltype(api.sgd_norm))p[8];
-    api.last_error = (decltype(api.last_error))p[9];
+    api.sgd_norm_host = (decltype(api.sgd_norm_host))p[9]; api.last_error = (decltype(api.last_error))p[10];
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }

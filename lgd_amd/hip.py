@@ -136,6 +136,7 @@ SIGNATURES = {
     "lgd_grad_clip": (c_i, [c_fp, c_i, c_i, c_f, c_fp, c_fp, c_fp]),
     "lgd_sgd_norm_ws_bytes": (c_sz, [c_i]),
     "lgd_sgd_norm_step": (c_i, [c_fp, c_fp, c_i, c_i, c_fp, c_fp, c_i, c_i, c_f, c_fp, c_fp, c_fp]),
+    "lgd_sgd_norm_step_host": (c_i, [c_fp, c_fp, c_i, c_i, c_fp, c_fp, c_i, c_i, c_f, c_fp, c_fp, c_fp]),
     "lgd_gn_act_ws_bytes": (c_sz, [c_fp, c_i, c_i, c_i, c_i, c_i, c_i]),
     "lgd_gn_act_fwd": (c_i, [c_fp, c_fp, c_i, c_i, c_i, c_i, c_i, c_fp, c_fp, c_i, ctypes.c_double, c_i, c_fp, c_fp, c_fp, c_fp]),
     "lgd_gn_act_bwd": (c_i, [c_fp, c_fp, c_fp, c_i, c_i, c_i, c_i, c_i, c_fp, c_fp, c_i, c_i, c_fp, c_fp, c_fp, c_fp, c_fp, c_fp]),
@@ -188,7 +189,7 @@ def load():
 
 _HOST_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "_lgd_host.so")
 _HOST_ENTRIES = ("lgd_gn_act_ws_bytes", "lgd_gn_act_fwd", "lgd_gn_act_bwd", "lgd_grad_norm_ws_bytes", "lgd_grad_norm", "lgd_grad_clip",
-                 "lgd_sgd_clip_step", "lgd_sgd_norm_ws_bytes", "lgd_sgd_norm_step", "lgd_last_error")
+                 "lgd_sgd_clip_step", "lgd_sgd_norm_ws_bytes", "lgd_sgd_norm_step", "lgd_sgd_norm_step_host", "lgd_last_error")
 _host = None
 
 

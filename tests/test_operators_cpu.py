@@ -126,6 +126,11 @@ def test_c_entries_refuse_bad_arguments(lib):
                 dict(m=float("nan")), dict(ws=None), dict(out=None), dict(o=hip.int_array([0, 3, 2])), dict(b=hip.int_array([0, 4, 3])),
                 dict(o=hip.int_array([1, 1, 2])), dict(o=hip.int_array([0, 0, 2]), b=hip.int_array([0, 1, 3]))):
         assert step(**bad) == -1, bad
+    recs = (ctypes.c_uint8 * (48 * 73))()   # the form with the table in host memory: refused before anything of it is used
+    host = lambda tab=recs, nt=2, nb=3, o=off, b=blk, ng=2, kind=0, m=1.0, ws=one, out=one: lib.lgd_sgd_norm_step_host(  # noqa: E731
+        tab, b, nt, nb, o, b, ng, kind, m, ws, out, None)
+    for bad in (dict(tab=None), dict(nt=0), dict(nt=73), dict(nb=4), dict(b=None), dict(o=None), dict(ng=17), dict(kind=3), dict(m=-1.0), dict(ws=None), dict(out=None)):
+        assert host(**bad) == -1, bad
     assert lib.lgd_sgd_norm_ws_bytes(0) == 0 and lib.lgd_sgd_norm_ws_bytes(2) > 0
 
 

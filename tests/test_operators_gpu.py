@@ -533,6 +533,62 @@ def test_fused_step_clips_by_norm(p):
     assert torch.equal(high.total_norms, torch.zeros(2, device=DEV)) and all(torch.equal(c, d) for c, d in zip(pc, pd))
 
 
+@pytest.mark.parametrize("count", [72, 73, 300])
+def test_fused_step_by_norm_many_tensors(count):
+    """tables that travel in the kernels' arguments and tables in device memory; three optimizers, the last without a gradient; the set of parameters that
+    have a gradient changes between the steps, and a state dict is loaded"""
+    from lgd_amd import optim
+    sizes = [1 + (i * 397) % 5003 for i in range(count)]
+
+    def make():
+        g = torch.Generator().manual_seed(14)
+        ps = [torch.nn.Parameter(torch.randn(n, generator=g).to(DEV)) for n in sizes]
+        extra = torch.nn.Parameter(torch.ones(3, device=DEV))
+        return ps, [torch.optim.SGD(ps[:count // 3], 0.02, momentum=0.9, weight_decay=1e-4), torch.optim.SGD(ps[count // 3:], 0.05, momentum=0.8),
+                    torch.optim.SGD([extra], 0.1)]
+    (pa, oa), (pb, ob) = make(), make()
+    fused = optim.FusedClipSGD(ob, clip_norm=5.0)
+    for step in range(4):
+        for i, (a, b) in enumerate(zip(pa, pb)):
+            a.grad = b.grad = None
+            if step != 1 or i % 2:
+                a.grad = _rand((sizes[i],), 70 * step + i).float().to(DEV)
+                b.grad = a.grad.clone()
+        if step == 3:
+            for o in ob:
+                o.load_state_dict(o.state_dict())
+        want = [float(torch.nn.utils.clip_grad_norm_([q for g in o.param_groups for q in g["params"]], 5.0)) for o in oa]
+        for o in oa:
+            o.step()
+        version = pb[1]._version
+        fused.step()
+        assert pb[1]._version > version
+        assert all(abs(float(x) - w) <= 1e-5 * w for x, w in zip(fused.total_norms, want))
+        for i, (a, b) in enumerate(zip(pa, pb)):
+            assert torch.allclose(a, b, rtol=2e-5, atol=2e-6), (step, i)
+            assert a.grad is None or torch.allclose(a.grad, b.grad, rtol=2e-5, atol=1e-9)
+
+
+def test_fused_step_refusals():
+    """gradients that share memory (by norm), strided gradients and strided parameters; nothing has been changed when the step refuses"""
+    from lgd_amd import hip, optim
+    p, q = (torch.nn.Parameter(torch.ones(8, 4, device=DEV)) for _ in range(2))
+    buf = torch.ones(48, device=DEV)
+    f = optim.FusedClipSGD([torch.optim.SGD([p, q], 0.1)], clip_norm=1.0)
+    p.grad, q.grad = buf[:32].view(8, 4), buf[16:].view(8, 4)
+    with pytest.raises(hip.LgdHipError, match="share memory"):
+        f.step()
+    p.grad, q.grad = torch.ones(8, 4, device=DEV), torch.ones(4, 8, device=DEV).t()
+    with pytest.raises(hip.LgdHipError, match="contiguous fp32 gradients"):
+        f.step()
+    assert torch.equal(p, torch.ones_like(p)) and torch.equal(q, torch.ones_like(q)) and torch.equal(buf, torch.ones_like(buf))
+    s = torch.nn.Parameter(torch.ones(4, 8, device=DEV).t())
+    f = optim.FusedClipSGD([torch.optim.SGD([s], 0.1)], clip_norm=1.0)
+    s.grad = torch.ones(8, 4, device=DEV)
+    with pytest.raises(hip.LgdHipError, match="contiguous"):
+        f.step()
+
+
 def test_fused_step_by_norm_is_not_captured():
     from lgd_amd import hip, optim
     p = torch.nn.Parameter(torch.ones(8, device=DEV))
