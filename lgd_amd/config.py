@@ -192,6 +192,7 @@ def get_cfg():
         SOLVER=dict(IMS_PER_BATCH=16, BASE_LR=0.001, STEPS=(30000,), MAX_ITER=40000, MOMENTUM=0.9, NESTEROV=False,
                     WEIGHT_DECAY=1e-4, GAMMA=0.1, WARMUP_FACTOR=1e-3, WARMUP_ITERS=1000, WARMUP_METHOD="linear",
                     CHECKPOINT_PERIOD=5000,
+                    # CLIP_TYPE "value" (element-wise), "norm" (each parameter's), "full_model" (each optimizer's whole gradient)
                     CLIP_GRADIENTS=dict(ENABLED=False, CLIP_TYPE="value", CLIP_VALUE=1.0, NORM_TYPE=2.0)),
         TEST=dict(EVAL_PERIOD=0, DETECTIONS_PER_IMAGE=100),
     ))

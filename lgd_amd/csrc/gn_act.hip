@@ -26,6 +26,8 @@ constexpr int kGaMax = 320;            // of the streaming kernels: 192, 256 or 
 constexpr int kGaFusedG = 512;         // groups of a fused call at most (its statistics lie in LDS) ...
 constexpr int kGaFusedRecords = 8192;  // ... and records x groups of a sample (64 - 128 KB that every workgroup of the apply kernel reads from the L2)
 
+constexpr int kGaParamC = 16;          // channels of a workgroup that makes dgamma and dbeta
+
 struct GaArgs {
     const void* x[LGD_MAX_LEVELS];
     const void* dy[LGD_MAX_LEVELS];
@@ -499,7 +501,6 @@ __global__ __launch_bounds__(256) void ga_param_kernel(GaArgs a) {
 }
 
 // dgamma, dbeta of 16 channels: the channel sums of every chunk of every (map, sample); 16 channels x NT / 16 slices of the records
-constexpr int kGaParamC = 16;
 __device__ __forceinline__ void ga_params(const GaArgs& a) {
     __shared__ double sh[kGaMax][2];
     const int c = blockIdx.x * kGaParamC + (threadIdx.x & 15), sl = threadIdx.x >> 4, slices = a.NT >> 4, n = a.wg0[LGD_MAX_LEVELS] * ga_per_chunk(a);
@@ -618,9 +619,11 @@ static int ga_plan(GaArgs& a, const int32_t* hw, int L, int B, int C, int G, int
         w += B * k;
         wf += B * (k < cap ? k : cap);
     }
-    if (w * rec > 0x3fffffffLL || (long long)L * B * G > 0x7fffffffLL) return LGD_EINVAL;
     // one kernel less where the records are few enough without leaving the chip short of workgroups
     a.fused = G <= kGaFusedG && cap >= 1 && (wf == w || wf >= 384);
+    if ((w + C / kGaParamC + 1) * a.NT > 0xffffffffLL || w * a.nCB > 0x3fffffffLL || (!a.fused && (long long)L * B * G * kGaThreads > 0xffffffffLL) ||
+        (long long)L * B * G > 0x3fffffffLL)
+        return LGD_EINVAL;   // (threads of a launch; 32-bit numbers of records and statistics)
     w = 0;
     for (int l = 0; l < L; ++l) {
         if (a.fused && a.K[l] > cap) a.K[l] = (int)cap;

@@ -132,7 +132,8 @@ __global__ __launch_bounds__(kSlabThreads) void slab_fwd_kernel(SlabArgs a) {
     const char* px = reinterpret_cast<const char*>(static_cast<const T*>(a.x[q.l]) + (size_t)q.b * HW * a.C);
     char* po = reinterpret_cast<char*>(static_cast<T*>(a.out[q.l]) + (size_t)q.b * HW * a.C);
     // atoms u <= full of all threads are rows of the slab but for the last one's tail
-    const int full = HW / a.rows, step = a.rows * a.C * (int)sizeof(T), mine = row0 >= a.rows ? 0 : row0 < HW - full * a.rows ? full + 1 : full;
+    const unsigned step = (unsigned)a.rows * (unsigned)a.C * (unsigned)sizeof(T);
+    const int full = HW / a.rows, mine = row0 >= a.rows ? 0 : row0 < HW - full * a.rows ? full + 1 : full;
     SlabReg<VW> x[N];
     {
         unsigned e = ((unsigned)row0 * a.C + c0) * (unsigned)sizeof(T);
@@ -238,7 +239,8 @@ __device__ __forceinline__ void slab_bwd_body(const SlabArgs& a, const SlabWhere
     const char* px = reinterpret_cast<const char*>(static_cast<const T*>(a.x[q.l]) + (size_t)q.b * HW * a.C);
     const char* pd = reinterpret_cast<const char*>(static_cast<const T*>(a.dy[q.l]) + (size_t)q.b * HW * a.C);
     // atoms u <= full of all threads are rows of the slab but for the last one's tail
-    const int full = HW / a.rows, step = a.rows * a.C * (int)sizeof(T), mine = row0 >= a.rows ? 0 : row0 < HW - full * a.rows ? full + 1 : full;
+    const unsigned step = (unsigned)a.rows * (unsigned)a.C * (unsigned)sizeof(T);
+    const int full = HW / a.rows, mine = row0 >= a.rows ? 0 : row0 < HW - full * a.rows ? full + 1 : full;
     SlabReg<VW> x[N], d[N];
     {
         unsigned e = ((unsigned)row0 * a.C + c0) * (unsigned)sizeof(T);
@@ -387,7 +389,7 @@ static bool slab_plan(SlabArgs& a, SlabPlan& p, const GaCall& c) {
             a.dy[l] = c.dy ? c.dy[l] : nullptr; a.out[l] = c.out ? c.out[l] : nullptr;
             a.HW[l] = c.hw[2 * l] * c.hw[2 * l + 1];
             w += ((long long)a.cnt + 7) / 8 * 8;
-            if (w > 0x3fffffffLL) return false;
+            if (w * p.NT > 0xffffffffLL) return false;   // threads of a launch
         }
         a.wg0[LGD_MAX_LEVELS] = (int)w;
         a.act = c.act; a.ptype = c.ptype; a.eps = c.eps; a.gamma = c.gamma; a.beta = c.beta; a.stats = c.stats; a.csum = c.csum;

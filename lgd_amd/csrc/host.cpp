@@ -92,17 +92,21 @@ void gn_check(const variable_list& xs, int64_t groups, const Tensor& w, const Te
     if (xs.size() > LGD_MAX_LEVELS) refuse("at most ", LGD_MAX_LEVELS, " maps per call (LGD_MAX_LEVELS), got ", xs.size());
     if (type_code(x0) < 0) refuse("group_norm_act takes fp32, bf16 or fp16 maps, got ", x0.scalar_type());
     for (const Tensor& x : xs) {
-        if (x.dim() != 4 || x0.dim() != 4 || x.size(0) != x0.size(0) || x.size(1) != x0.size(1)) refuse("maps of one call are (B,C,H_l,W_l) with the same B and C, got ", x0.sizes(), " and ", x.sizes());
+        if (x.dim() != 4 || x0.dim() != 4 || x.size(0) != x0.size(0) || x.size(1) != x0.size(1))
+            refuse("maps of one call are (B,C,H_l,W_l) with the same B and C, got ", x0.sizes(), " and ", x.sizes());
         if (x.scalar_type() != x0.scalar_type() || x.device() != x0.device() || x.layout() != at::kStrided)
-            refuse("maps of one call are strided, of one type and on one device, got ", x.layout(), " ", x.scalar_type(), " ", x.device(), " beside ", x0.scalar_type(), " ", x0.device());
+            refuse("maps of one call are strided, of one type and on one device, got ", x.layout(), " ", x.scalar_type(), " ", x.device(), " beside ",
+                   x0.scalar_type(), " ", x0.device());
         for (int d = 0; d < 4; ++d) if (x.size(d) > INT32_MAX) refuse("a map's sizes are below 2^31, got ", x.sizes());
     }
     const int64_t C = x0.size(1);
     if (groups < 1 || C < 1 || groups > C || C % groups) refuse(C, " channels do not split into ", groups, " groups");
     for (const Tensor* p : {&w, &b})
         if (p->defined() && (type_code(*p) < 0 || p->dim() != 1 || p->size(0) != C || p->device() != x0.device() || p->layout() != at::kStrided))
-            refuse(p == &w ? "weight" : "bias", " must be ", C, " fp32, bf16 or fp16 values on ", x0.device(), ", got ", p->sizes(), " ", p->scalar_type(), " on ", p->device());
-    if (w.defined() && b.defined() && w.scalar_type() != b.scalar_type()) refuse("weight and bias have one type, got ", w.scalar_type(), " and ", b.scalar_type());
+            refuse(p == &w ? "weight" : "bias", " must be ", C, " fp32, bf16 or fp16 values on ", x0.device(), ", got ", p->sizes(), " ",
+                   p->scalar_type(), " on ", p->device());
+    if (w.defined() && b.defined() && w.scalar_type() != b.scalar_type())
+        refuse("weight and bias have one type, got ", w.scalar_type(), " and ", b.scalar_type());
 }
 
 // xs dense, w and b contiguous; stats: kept for a backward.  Below autograd
@@ -114,7 +118,7 @@ variable_list gn_forward(const variable_list& xs, int groups, int act, double ep
     if (c.L == 0) return ys;
     const c10::DeviceGuard guard(xs[0].device());
     const size_t n = api.gn_ws(c.hw.data(), c.L, c.B, c.C, groups, c.type, 0);
-    if (n == (size_t)-1) refuse("group_norm_act: maps of 2^31 elements per sample or more are not supported");
+    if (n == (size_t)-1) refuse("group_norm_act: 2^31 elements per sample, or 2^30 groups of all maps and samples, or more are not supported");
     const int64_t words = 2LL * c.L * c.B * groups;
     const auto f64 = xs[0].options().dtype(at::kDouble).memory_format(at::MemoryFormat::Contiguous);
     // one allocation, unless the statistics outlive the workspace
@@ -150,6 +154,19 @@ struct GnBackward : public Node {
         stats.reset();
         released = true;
     }
+    // A leaf whose gradient accumulator belongs to an older graph, made on another stream, would have the engine make that stream wait inside the capture:
+    // an error that ends the process.  Refused before it gets there
+    void refuse_capture() {
+        if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+        const c10::StreamId here = c10::hip::getCurrentHIPStream().id();
+        for (const auto& e : next_edges()) {
+            if (!e.function || e.function->num_outputs() != 0) continue;   // (accumulators have no next functions)
+            const auto s = e.function->stream();
+            if (s && s->id() != here)
+                throw std::runtime_error("group_norm_act: a leaf of this captured backward is held by a graph that was made on another stream; "
+                                         "release that graph, or capture with leaves of its own");
+        }
+    }
     variable_list apply(variable_list&& dys) override {
         TORCH_CHECK(!released, "group_norm_act: the graph has been freed; backward a second time needs retain_graph=True the first time");
         const bool again = at::GradMode::is_enabled();   // create_graph
@@ -160,13 +177,16 @@ struct GnBackward : public Node {
         bool any = false;
         for (const Tensor& d : dys) any = any || d.defined();
         if (!any) return out;
+        refuse_capture();
         {
             at::AutoDispatchBelowADInplaceOrView below;
             run(xs, wv, bv, dys, out);
         }
         if (again) {
             torch::autograd::edge_list edges;
-            auto edge = [&](const Tensor& t) { if (t.defined() && t.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(t)); };
+            auto edge = [&](const Tensor& t) {
+                if (t.defined() && t.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(t));
+            };
             for (const Tensor& t : xs) edge(t);
             edge(wv); edge(bv);
             for (const Tensor& t : dys) edge(t);
@@ -178,8 +198,11 @@ struct GnBackward : public Node {
         }
         return out;
     }
-    void run(const variable_list& xs, const Tensor& wv, const Tensor& bv, const variable_list& dys, variable_list& out) {
-        const size_t nx = xs.size();
+    void run(const variable_list& saved, const Tensor& w0, const Tensor& b0, const variable_list& dys, variable_list& out) {
+        const size_t nx = saved.size();
+        variable_list xs;   // (hooks on saved tensors may hand them back in another order)
+        for (const Tensor& x : saved) xs.push_back(dense(x));
+        const Tensor wv = w0.defined() ? w0.contiguous() : w0, bv = b0.defined() ? b0.contiguous() : b0;
         bool want_x = false;
         for (size_t i = 0; i < nx; ++i) want_x = want_x || task_should_compute_output(i);
         Tensor dw, db;
@@ -299,7 +322,8 @@ Tensor norm_of(const std::vector<Tensor>& ts, int norm_type, bool clip, double m
     for (const Tensor& t : ts) {
         const int type = type_code(t);
         if (t.layout() != at::kStrided || type < 0 || t.device() != dev)
-            refuse("gradient norms take strided fp32, bf16 or fp16 tensors on one device, got ", t.layout(), " ", t.scalar_type(), " ", t.device(), " (the first is on ", dev, ")");
+            refuse("gradient norms take strided fp32, bf16 or fp16 tensors on one device, got ",
+                   t.layout(), " ", t.scalar_type(), " ", t.device(), " (the first is on ", dev, ")");
         flat.push_back(t.is_non_overlapping_and_dense() ? t : t.contiguous());   // any dense order is one run of memory
         rec.push_back({flat.back().data_ptr(), t.numel(), type, 0});
     }
@@ -334,7 +358,8 @@ struct SgdPlan {
 };
 enum class Sgd { kDone, kOtherSet, kNotGpu };
 
-Sgd sgd_step(PyObject* params, PyObject* momenta, const SgdPlan& plan, const std::vector<float>& hyper, bool by_norm, int norm_type, double clip, Tensor& norms) {
+Sgd sgd_step(PyObject* params, PyObject* momenta, const SgdPlan& plan, const std::vector<float>& hyper, bool by_norm, int norm_type, double clip,
+             Tensor& norms) {
     const int n = (int)PyList_GET_SIZE(params), k = plan.k;
     std::vector<Tensor> ps, gs, ms;
     ps.reserve(k); gs.reserve(k); ms.reserve(k);
@@ -494,7 +519,8 @@ PyObject* py_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // plan: six bytes objects in the order of SgdPlan
 PyObject* py_sgd_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 6 || !PyList_Check(a[0]) || !PyList_Check(a[1]) || PyList_GET_SIZE(a[0]) != PyList_GET_SIZE(a[1]) || !PyTuple_Check(a[2]) || PyTuple_GET_SIZE(a[2]) != 6 || !PyList_Check(a[3])) {
+    if (n != 6 || !PyList_Check(a[0]) || !PyList_Check(a[1]) || PyList_GET_SIZE(a[0]) != PyList_GET_SIZE(a[1]) || !PyTuple_Check(a[2]) ||
+        PyTuple_GET_SIZE(a[2]) != 6 || !PyList_Check(a[3])) {
         PyErr_SetString(PyExc_TypeError, "sgd_step(list, list, plan, list, norm code, clip)");
         return nullptr;
     }
@@ -505,20 +531,22 @@ PyObject* py_sgd_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (!PyBytes_Check(b)) { PyErr_SetString(PyExc_TypeError, "a plan holds bytes"); return nullptr; }
         part[i] = PyBytes_AS_STRING(b); size[i] = PyBytes_GET_SIZE(b);
     }
-    SgdPlan plan = {static_cast<const int32_t*>(part[0]), static_cast<const lgd_sgd_tensor*>(part[1]), static_cast<const int32_t*>(part[2]), static_cast<const int32_t*>(part[3]),
-                    static_cast<const int32_t*>(part[4]), static_cast<const int32_t*>(part[5]), (int)(size[0] / 4), (int)(size[4] / 4) - 1};
+    const auto ints = [&](int i) { return static_cast<const int32_t*>(part[i]); };
+    const SgdPlan plan = {ints(0), static_cast<const lgd_sgd_tensor*>(part[1]), ints(2), ints(3), ints(4), ints(5), (int)(size[0] / 4), (int)(size[4] / 4) - 1};
     std::vector<float> hyper;
     for (Py_ssize_t i = 0; i < PyList_GET_SIZE(a[3]); ++i) hyper.push_back((float)PyFloat_AsDouble(PyList_GET_ITEM(a[3], i)));
     const bool by_norm = a[4] != Py_None;
     const long code = by_norm ? PyLong_AsLong(a[4]) : 0;
     const double clip = PyFloat_AsDouble(a[5]);
     if (PyErr_Occurred()) return nullptr;
-    bool fits = plan.k > 0 && size[1] == (Py_ssize_t)(plan.k * sizeof(lgd_sgd_tensor)) && size[2] == 4 * (plan.k + 1) && size[3] == 4 * plan.k && plan.groups > 0 && size[5] == size[4];
+    bool fits = plan.k > 0 && size[1] == (Py_ssize_t)(plan.k * sizeof(lgd_sgd_tensor)) && size[2] == 4 * (plan.k + 1) && size[3] == 4 * plan.k &&
+                plan.groups > 0 && size[5] == size[4];
     for (Py_ssize_t i = 0; fits && i < PyList_GET_SIZE(a[0]); ++i) fits = THPVariable_Check(PyList_GET_ITEM(a[0], i));
     for (int j = 0; fits && j < plan.k; ++j) {
         const Py_ssize_t i = plan.rows[j];
-        fits = i >= 0 && i < PyList_GET_SIZE(a[0]) && THPVariable_Check(PyList_GET_ITEM(a[1], i)) && plan.set[j] >= 0 && 3 * (size_t)plan.set[j] + 3 <= hyper.size() &&
-               plan.table[j].n == THPVariable_Unpack(PyList_GET_ITEM(a[0], i)).numel() && plan.table[j].n == THPVariable_Unpack(PyList_GET_ITEM(a[1], i)).numel();
+        fits = i >= 0 && i < PyList_GET_SIZE(a[0]) && THPVariable_Check(PyList_GET_ITEM(a[1], i)) && plan.set[j] >= 0 &&
+               3 * (size_t)plan.set[j] + 3 <= hyper.size() && plan.table[j].n == THPVariable_Unpack(PyList_GET_ITEM(a[0], i)).numel() &&
+               plan.table[j].n == THPVariable_Unpack(PyList_GET_ITEM(a[1], i)).numel();
     }
     if (!fits) { PyErr_SetString(PyExc_ValueError, "the plan does not fit the lists"); return nullptr; }
     try {

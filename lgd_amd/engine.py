@@ -286,12 +286,12 @@ class Trainer:
     def _clip(self):
         """detectron2 maybe_add_gradient_clipping: per PARAMETER, CLIP_TYPE 'value' (default, CLIP_VALUE 1.0) = element-wise
         clamp, 'norm' = clip_grad_norm_ of each parameter on its own [d2-memory]; multi-tensor forms, no host sync.  'full_model' = by the
-        norm of each optimizer's whole gradient (optim.clip_grad_norm_ on the GPU, torch's on the CPU)."""
+        norm of each optimizer's whole gradient (optim.clip_grad_norm_ on the GPU; torch's on the CPU and for norms other than 1, 2 and inf)."""
         if self.clip.CLIP_TYPE == "full_model":
+            from . import optim
             for o in (self.stu_optimizer, self.tea_optimizer):
                 params = [p for g in o.param_groups for p in g["params"] if p.grad is not None]
-                if params and params[0].is_cuda:
-                    from . import optim
+                if params and params[0].is_cuda and optim.has_norm(self.clip.NORM_TYPE):
                     optim.clip_grad_norm_(params, self.clip.CLIP_VALUE, self.clip.NORM_TYPE)
                 else:
                     torch.nn.utils.clip_grad_norm_(params, float(self.clip.CLIP_VALUE), float(self.clip.NORM_TYPE))

@@ -22,6 +22,10 @@ assert _TENSOR_DT.itemsize == 48
 _NORMS = {2.0: 0, 1.0: 1, float("inf"): 2}   # LGD_NORM_*
 
 
+def has_norm(norm_type):
+    return float(norm_type) in _NORMS
+
+
 def _norm_code(norm_type):
     code = _NORMS.get(float(norm_type))
     if code is None:
@@ -64,7 +68,7 @@ def supported(optimizers, clip):
     else stays on torch's own multi-tensor path."""
     if clip.ENABLED and clip.CLIP_TYPE not in ("value", "full_model"):
         return False
-    if clip.ENABLED and clip.CLIP_TYPE == "full_model" and float(clip.NORM_TYPE) not in _NORMS:
+    if clip.ENABLED and clip.CLIP_TYPE == "full_model" and not has_norm(clip.NORM_TYPE):
         return False
     for o in optimizers:
         if type(o) is not torch.optim.SGD:

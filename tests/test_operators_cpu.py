@@ -106,6 +106,9 @@ def test_c_entries_refuse_bad_arguments(lib):
     assert bytes_of(big, 1, 0) == bytes_of(big, 1, 1) == ctypes.c_size_t(-1).value and bytes_of(hip.int_array([80, 800]), 1, 0) > 0
     assert bytes_of(hw, 2, 0) == 0 and bytes_of(hw, 1, 1) == 0 and bytes_of(hw, 2, 1) > 0   # small: no workspace but for the parameters' gradients
 
+    one_px = hip.int_array([1, 1])   # more workgroups or statistics than a launch numbers
+    assert lib.lgd_gn_act_ws_bytes(one_px, 1, 1 << 25, 64, 64, 0, 0) == lib.lgd_gn_act_ws_bytes(one_px, 1, 1 << 21, 520, 520, 0, 1) == ctypes.c_size_t(-1).value
+
     def norm(rec, n=1, kind=0, ws=one, out=one, clip=None):
         r = (hip.GradTensor * 1)(rec)
         if clip is not None:

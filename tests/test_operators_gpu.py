@@ -214,6 +214,41 @@ def test_group_norm_act_empty_and_partial_gradients():
         (g * x).sum().backward()
 
 
+def test_group_norm_act_saved_tensors_kept_elsewhere():
+    """what the backward needs, kept on the host in another memory order; the same map twice in one call; a second backward of a kept graph"""
+    from lgd_amd import ops
+    x, = _maps(2, 24, [(9, 11)], torch.float32, 31)
+    dys = _maps(2, 24, [(9, 11), (9, 11)], torch.float32, 32)
+    w, b = _params(24, torch.float32, 33)
+    x.requires_grad_(True)
+    ys = ops.group_norm_act([x, x], 6, w, b, act="silu")
+    want = torch.autograd.grad(ys, [x, w, b], dys, retain_graph=True)
+    assert all(torch.equal(g, a) for g, a in zip(torch.autograd.grad(ys, [x, w, b], dys), want))
+    with pytest.raises(RuntimeError, match="freed"):
+        torch.autograd.grad(ys, [x], dys)
+    one, two = (torch.autograd.grad(ops.group_norm_act([x], 6, w, b, act="silu"), [x], [dy])[0] for dy in dys)
+    assert torch.equal(one + two, want[0])
+    with torch.autograd.graph.save_on_cpu(pin_memory=True):
+        ys = ops.group_norm_act([x, x], 6, w, b, act="silu")
+    assert all(torch.equal(g, a) for g, a in zip(torch.autograd.grad(ys, [x, w, b], dys), want))
+
+
+def test_group_norm_act_captured_beside_an_eager_graph_of_the_same_leaves():
+    """refused before the engine makes the eager graph's stream wait inside the capture"""
+    from lgd_amd import ops
+    x, dy = _maps(1, 16, [(5, 5)], torch.float32, 41)[0].requires_grad_(True), _maps(1, 16, [(5, 5)], torch.float32, 42)[0]
+    w, b = _params(16, torch.float32, 43)
+    kept = ops.group_norm_act([x], 4, w, b)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="held by a graph"):
+        with torch.cuda.graph(graph):
+            torch.autograd.grad(ops.group_norm_act([x], 4, w, b), [x, w, b], [dy])
+    torch.cuda.synchronize()
+    want = torch.autograd.grad(kept, [x, w, b], [dy])
+    assert all(torch.isfinite(g).all() for g in want)
+
+
 @pytest.mark.parametrize("act", ["none", "relu", "silu"])
 def test_group_norm_act_not_finite_stays_in_its_group(act):
     """inf and NaN spoil their own (sample, group) as in torch, and nothing else"""
