@@ -13,6 +13,33 @@ __device__ __forceinline__ float ga_param(const void* p, int type, int c, float 
     if (type == LGD_BF16) return (float)static_cast<const __bf16*>(p)[c];
     return (float)static_cast<const _Float16*>(p)[c];
 }
+// the same for N channels as raw words, so that all the loads are on their way together (a load and its conversion per channel wait for each other:
+// 16 of them took 3 us of an 8 us kernel)
+template <int N> __device__ __forceinline__ void ga_param_words(const void* p, int type, const int (&c)[N], uint32_t (&w)[N]) {
+    if (!p) return;
+    if (type == LGD_F32) {
+        #pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = static_cast<const uint32_t*>(p)[c[i]];
+    } else {
+        #pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = static_cast<const uint16_t*>(p)[c[i]];
+    }
+}
+template <int N> __device__ __forceinline__ void ga_param_values(const void* p, int type, const uint32_t (&w)[N], float none, float (&v)[N]) {
+    if (!p) {
+        #pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = none;
+    } else if (type == LGD_F32) {
+        #pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = __builtin_bit_cast(float, w[i]);
+    } else if (type == LGD_BF16) {
+        #pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = __builtin_bit_cast(float, w[i] << 16);
+    } else {
+        #pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = (float)__builtin_bit_cast(_Float16, (uint16_t)w[i]);
+    }
+}
 __device__ __forceinline__ void ga_param_store(void* p, int type, int c, float v) {
     if (type == LGD_F32) static_cast<float*>(p)[c] = v;
     else if (type == LGD_BF16) static_cast<__bf16*>(p)[c] = (__bf16)v;
@@ -38,8 +65,7 @@ template <int ACT> __device__ __forceinline__ float ga_act(float z) {
 // The backward's constants of one channel (n = 1: of a lane; the mean and the inverse deviation belong to its group).  mean = hi + lo and
 // 1/deviation = r + rl are pairs of fp32 words: xh = (x - hi) r - lo r is as good as the fp64 form (x - hi is exact near the mean)
 struct GaGroup { float hi, lo, r, rl, nlr; };
-__device__ __forceinline__ GaGroup ga_group(const double* st, int g) {
-    const double m = st[2 * g], r = st[2 * g + 1];
+__device__ __forceinline__ GaGroup ga_group(double m, double r) {
     GaGroup k;
     k.hi = (float)m; k.lo = (float)(m - (double)k.hi);
     k.r = (float)r; k.rl = (float)(r - (double)k.r);

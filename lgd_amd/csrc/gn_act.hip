@@ -15,12 +15,15 @@
 // thread's rows of a chunk (<= a few hundred terms) and its workgroup, fp64 from there on.  Outputs are rounded once (fp32 -> 16 bits).
 #include "gn_act.h"
 
+#include <type_traits>
+
 namespace lgd {
 
 // Workgroups of a streaming call, about: two for every CU, in step.  8 x 320 x 256 x 256 bf16, forward / backward us: 512 168 / 291, 768 197 / 345 (three on
 // some CUs, four on others), 1024 177 / 299
 constexpr int kGaWorkgroups = 512;
 constexpr int kGaU = 4, kGaUB = 2;     // vectors (of x; of x and dy each) of a thread in flight
+constexpr int kGaRecordsU = 8;         // records of a thread in flight
 constexpr int kGaThreads = 256;        // of the kernels in between
 constexpr int kGaMax = 320;            // of the streaming kernels: 192, 256 or 320, whichever has a vector for most of its threads
 constexpr int kGaFusedG = 512;         // groups of a fused call at most (its statistics lie in LDS) ...
@@ -173,67 +176,78 @@ template <typename T> __device__ __forceinline__ void ga_store_n(T* p, const lgd
     for (int i = 0; i < Vec16<T>::V; ++i) if (i < count) p[i] = tmp[i];
 }
 
-// ---- sums of a workgroup: every thread brings V pairs (one per position of the super-row); fixed-order tree over the R super-rows, result in
-// sh[position][2] for the positions of this column block.  sh holds kGaMax * V pairs.
-template <int V, typename A>
-__device__ __forceinline__ void ga_block_positions(const GaArgs& a, const GaThread& t, A (&s0)[V], A (&s1)[V], A* sh) {
-    const int r = t.r, col = threadIdx.x - r * a.cols;
-    int half = 1;
-    while (half < a.R) half <<= 1;
-    for (half >>= 1; half >= 1; half >>= 1) {
-        if (t.on && r >= half && r < 2 * half) {
-            A* p = sh + (long)((r - half) * a.cols + col) * V * 2;
-            #pragma unroll
-            for (int i = 0; i < V; ++i) { p[2 * i] = s0[i]; p[2 * i + 1] = s1[i]; }
-        }
-        __syncthreads();
-        if (t.on && r < half && r + half < a.R) {
-            const A* p = sh + (long)(r * a.cols + col) * V * 2;
-            #pragma unroll
-            for (int i = 0; i < V; ++i) { s0[i] += p[2 * i]; s1[i] += p[2 * i + 1]; }
-        }
-        __syncthreads();
-    }
-    if (t.on && r == 0) {
-        A* p = sh + (long)col * V * 2;
-        #pragma unroll
-        for (int i = 0; i < V; ++i) { p[2 * i] = s0[i]; p[2 * i + 1] = s1[i]; }
-    }
-    __syncthreads();
-}
+// Pieces.  W = gcd(cg, V) consecutive lanes of a vector lie in one group (groups, rows and vectors all end at multiples of W), so a thread holds
+// S = V / W pieces: V = 8: one for groups of 8, 16, ... channels, two for 20, four for 30, eight for odd ones.
 
-// sums over the n terms of each of ng groups: value(g, i, k) of term i, k in {0, 1}; put(2 g + k, sum).  Few groups are split over the workgroup (a
-// thread walking a whole group alone took 12 us at 512 channels), the parts meet in a tree.  Barriers inside
-template <typename Value, typename Put>
-__device__ __forceinline__ void ga_block_groups(int nt, int ng, int n, Value value, Put put) {
-    __shared__ double tmp[kGaMax];
-    const int outs = 2 * ng;
-    if (outs > nt / 2) {
-        for (int j = threadIdx.x; j < outs; j += nt) {
-            double s = 0.0;
-            for (int i = 0; i < n; ++i) s += value(j >> 1, i, j & 1);
-            put(j, s);
+// ---- sums of a workgroup: pairs that the threads left in LDS, n bins of rows x per terms each; term(bin, r, c) -> the pair, put(bin, s0, s1).  Few bins
+// are split over the threads, neighbours taking neighbouring terms, and joined eight at a time in a fixed order.  Barriers inside, none in front
+template <typename Term, typename Put>
+__device__ __forceinline__ void ga_bins(int nt, int n, int rows, int per, Term term, Put put) {
+    __shared__ double2 tmp[kGaMax];
+    const int terms = rows * per;
+    int m = 1;   // threads of a bin
+    while (2 * m * n <= nt && m < terms) m <<= 1;
+    if (m == 1) {
+        for (int j = threadIdx.x; j < n; j += nt) {
+            double s0 = 0.0, s1 = 0.0;
+            for (int r = 0; r < rows; ++r)
+                for (int c = 0; c < per; ++c) { const auto v = term(j, r, c); s0 += (double)v.x; s1 += (double)v.y; }
+            put(j, s0, s1);
         }
         return;
     }
-    int slices = 1;
-    while (2 * slices * outs <= nt) slices <<= 1;
-    const int sl = threadIdx.x / outs, j = threadIdx.x - sl * outs;
-    double s = 0.0;
-    if (sl < slices) for (int i = sl; i < n; i += slices) s += value(j >> 1, i, j & 1);
-    for (slices >>= 1; slices >= 1; slices >>= 1) {
-        if (sl >= slices && sl < 2 * slices) tmp[threadIdx.x - slices * outs] = s;
-        __syncthreads();
-        if (sl < slices) s += tmp[threadIdx.x];
-        __syncthreads();
+    const int j = threadIdx.x / m, first = threadIdx.x & (m - 1);
+    double s0 = 0.0, s1 = 0.0;
+    if (j < n) {
+        const int dr = m / per, dc = m - dr * per;
+        for (int r = first / per, c = first - r * per; r < rows;) {
+            const auto v = term(j, r, c);
+            s0 += (double)v.x; s1 += (double)v.y;
+            r += dr; c += dc;
+            if (c >= per) { c -= per; ++r; }
+        }
     }
-    if (sl == 0) put(j, s);
+    __syncthreads();   // (tmp may be in use by an earlier call)
+    tmp[threadIdx.x] = make_double2(s0, s1);
+    for (;;) {
+        __syncthreads();
+        const int next = m > 8 ? m >> 3 : 1, step = m / next;
+        const bool on = (int)threadIdx.x < n * next;
+        const int bin = threadIdx.x / next, k = threadIdx.x - bin * next;
+        if (on) {
+            s0 = s1 = 0.0;
+            for (int i = 0; i < step; ++i) { const double2 v = tmp[bin * m + k + i * next]; s0 += v.x; s1 += v.y; }
+        }
+        if (next == 1) {
+            if (on) put(bin, s0, s1);
+            return;
+        }
+        __syncthreads();
+        if (on) tmp[threadIdx.x] = make_double2(s0, s1);
+        m = next;
+    }
 }
 
-template <typename T, bool UG>
+constexpr int kGaPad = kGaMax + 1;   // pairs between the pieces of a thread: neighbouring threads and neighbouring pieces lie on different banks
+
+// the groups' sums of a column block out of the threads' pieces sh[piece][thread]
+template <int V, int S, typename P2, typename Put>
+__device__ __forceinline__ void ga_piece_groups(const GaArgs& a, const GaBlock& blk, const P2* sh, Put put) {
+    constexpr int W = V / S;
+    const int per = a.cg / W, Cp = a.C / W, np = blk.np / W, shift = blk.shift / W;
+    ga_bins(a.NT, blk.ng, a.R, per, [&](int g, int r, int c) {
+        int o = (blk.g0 + g) * per + c - shift;
+        if (o < 0) o += Cp;
+        P2 s = {};
+        for (; o < np; o += Cp) { const P2 v = sh[(o & (S - 1)) * kGaPad + r * a.cols + o / S]; s.x += v.x; s.y += v.y; }
+        return s;
+    }, put);
+}
+
+template <typename T, int S>
 __global__ __launch_bounds__(kGaMax) void ga_stats_kernel(GaArgs a) {
-    constexpr int V = Vec16<T>::V, S = UG ? 1 : V;
-    __shared__ double sh[kGaMax * S * 2];
+    constexpr int V = Vec16<T>::V, W = V / S;
+    __shared__ double2 sh[S * kGaPad];
     const GaWhere q = ga_locate(a, blockIdx.x);
     const int E = a.E[q.l];
     const GaThread t = ga_thread<V>(a, E);
@@ -250,26 +264,14 @@ __global__ __launch_bounds__(kGaMax) void ga_stats_kernel(GaArgs a) {
             float f[V];
             Vec16<T>::unpack(v.x, f);
             #pragma unroll
-            for (int i = 0; i < V; ++i) { const double d = f[i]; s0[UG ? 0 : i] += d; s1[UG ? 0 : i] = fma(d, d, s1[UG ? 0 : i]); }
+            for (int i = 0; i < V; ++i) { const double d = f[i]; s0[i / W] += d; s1[i / W] = fma(d, d, s1[i / W]); }
         });
-    double* part = a.partd + ga_record(a) * a.G * 2;
+    double2* part = reinterpret_cast<double2*>(a.partd) + ga_record(a) * a.G;
     const GaBlock blk = ga_block<V>(a);
-    if constexpr (UG) {   // (not mixed) a thread's vectors lie in one group: its pair is all that the others need of it
-        sh[2 * threadIdx.x] = s0[0]; sh[2 * threadIdx.x + 1] = s1[0];
-        __syncthreads();
-        const int per = a.cg / V;
-        ga_block_groups(a.NT, blk.ng, a.R * per, [&](int g, int i, int k) {
-            const int r = i / per;
-            return sh[2 * (r * a.cols + g * per + i - r * per) + k];
-        }, [&](int j, double s) { part[2 * blk.g0 + j] = s; });
-    } else {
-        ga_block_positions<V, double>(a, t, s0, s1, sh);
-        ga_block_groups(a.NT, blk.ng, a.cg, [&](int g, int i, int k) {   // positions -> groups
-            double s = 0.0;
-            for (int o = blk.first((blk.g0 + g) * a.cg + i); o < blk.np; o += a.C) s += sh[2 * o + k];
-            return s;
-        }, [&](int j, double s) { part[2 * blk.g0 + j] = s; });
-    }
+    #pragma unroll
+    for (int i = 0; i < S; ++i) sh[i * kGaPad + threadIdx.x] = make_double2(s0[i], s1[i]);
+    __syncthreads();
+    ga_piece_groups<V, S>(a, blk, sh, [&](int g, double g0, double g1) { part[blk.g0 + g] = make_double2(g0, g1); });
 }
 
 // mean and 1 / sqrt(var + eps) of a group of n values with sums s0, s1
@@ -309,15 +311,13 @@ __device__ __forceinline__ void ga_records(int nt, const P2* __restrict__ p, int
         const int g = g0 + (threadIdx.x & (sub - 1));
         double s0 = 0.0, s1 = 0.0;
         if (g < gend && sl < slices) {
-            int k = sl;
-            for (; k + 3 * slices < K; k += 4 * slices) {
-                P2 v[4];
+            for (int k = sl; k < K; k += kGaRecordsU * slices) {
+                P2 v[kGaRecordsU];
                 #pragma unroll
-                for (int u = 0; u < 4; ++u) v[u] = p[(size_t)(k + u * slices) * G + g];
+                for (int u = 0; u < kGaRecordsU; ++u) { v[u] = P2{}; if (k + u * slices < K) v[u] = p[(size_t)(k + u * slices) * G + g]; }
                 #pragma unroll
-                for (int u = 0; u < 4; ++u) { s0 += (double)v[u].x; s1 += (double)v[u].y; }
+                for (int u = 0; u < kGaRecordsU; ++u) { s0 += (double)v[u].x; s1 += (double)v[u].y; }
             }
-            for (; k < K; k += slices) { const P2 v = p[(size_t)k * G + g]; s0 += (double)v.x; s1 += (double)v.y; }
         }
         if (slices > 1) {
             tmp[threadIdx.x][0] = s0; tmp[threadIdx.x][1] = s1;
@@ -340,6 +340,11 @@ __global__ __launch_bounds__(kGaMax) void ga_apply_kernel(GaArgs a) {
     const auto load = [&](unsigned e) { return GaX<T>{ga_stream(px + e)}; };
     GaWalk<V, kGaU, GaX<T>> walk;
     walk.begin(a, q, t, load);
+    int c[V], g[V];
+    ga_lanes<V>(a, t, [&](int i, int ci, int gi) { c[i] = ci; g[i] = gi; });
+    uint32_t wga[V] = {}, wbe[V] = {};   // (asked for in front of the barriers)
+    ga_param_words<V>(a.gamma, a.ptype, c, wga);
+    ga_param_words<V>(a.beta, a.ptype, c, wbe);
     double A[V], Bc[V];
     double* gst = a.stats + 2 * (size_t)(q.l * a.B + q.b) * a.G;
     const double* st = gst;
@@ -356,10 +361,13 @@ __global__ __launch_bounds__(kGaMax) void ga_apply_kernel(GaArgs a) {
         __syncthreads();
         st = sst;
     }
-    ga_lanes<V>(a, t, [&](int i, int c, int g) {
-        A[i] = st[2 * g + 1] * (double)ga_param(a.gamma, a.ptype, c, 1.f);
-        Bc[i] = fma(-st[2 * g], A[i], (double)ga_param(a.beta, a.ptype, c, 0.f));
-    });
+    {
+        float ga[V], be[V];
+        ga_param_values<V>(a.gamma, a.ptype, wga, 1.f, ga);
+        ga_param_values<V>(a.beta, a.ptype, wbe, 0.f, be);
+        #pragma unroll
+        for (int i = 0; i < V; ++i) { A[i] = st[2 * g[i] + 1] * (double)ga[i]; Bc[i] = fma(-st[2 * g[i]], A[i], (double)be[i]); }
+    }
     walk.run(a, q, t, E, load, [&](unsigned e, int n) { return GaX<T>{ga_load_part(px + e, n)}; },
         [&](const GaX<T>& v, unsigned e, int n) {
             float f[V];
@@ -370,24 +378,34 @@ __global__ __launch_bounds__(kGaMax) void ga_apply_kernel(GaArgs a) {
         });
 }
 
-// constants of a thread's V lanes; UG: V divides the channels of a group, so that a vector lies in one group
-template <int V, bool UG> struct GaCoef {
-    GaGroup grp[UG ? 1 : V];
+// constants of a thread's V lanes in S pieces
+template <int V, int S> struct GaCoef {
+    static constexpr int W = V / S;
+    GaGroup grp[S];
     float ga[V], be[V];
     __device__ __forceinline__ void fill(const GaArgs& a, const GaWhere& q, const GaThread& t) {
-        const double* st = a.stats + 2 * (size_t)(q.l * a.B + q.b) * a.G;
-        ga_lanes<V>(a, t, [&](int i, int c, int g) {
-            if (!UG || i == 0) grp[UG ? 0 : i] = ga_group(st, g);
-            ga[i] = ga_param(a.gamma, a.ptype, c, 1.f); be[i] = ga_param(a.beta, a.ptype, c, 0.f);
+        const double2* st = reinterpret_cast<const double2*>(a.stats) + (size_t)(q.l * a.B + q.b) * a.G;
+        int c[V];
+        double2 m[S];
+        ga_lanes<V>(a, t, [&](int i, int ci, int gi) {
+            c[i] = ci;
+            if (i % W == 0) m[i / W] = st[gi];
         });
+        uint32_t wga[V] = {}, wbe[V] = {};
+        ga_param_words<V>(a.gamma, a.ptype, c, wga);
+        ga_param_words<V>(a.beta, a.ptype, c, wbe);
+        ga_param_values<V>(a.gamma, a.ptype, wga, 1.f, ga);
+        ga_param_values<V>(a.beta, a.ptype, wbe, 0.f, be);
+        #pragma unroll
+        for (int i = 0; i < S; ++i) grp[i] = ga_group(m[i].x, m[i].y);
     }
-    __device__ __forceinline__ const GaGroup& at(int i) const { return grp[UG ? 0 : i]; }
+    __device__ __forceinline__ const GaGroup& at(int i) const { return grp[i / W]; }
 };
 
-template <typename T, int ACT, bool UG>
+template <typename T, int ACT, int S>
 __global__ __launch_bounds__(kGaMax) void ga_bwd_stats_kernel(GaArgs a) {
-    constexpr int V = Vec16<T>::V;
-    __shared__ float sh[kGaMax * V * 2];
+    constexpr int V = Vec16<T>::V, W = V / S;
+    __shared__ float2 sh[V * kGaPad], shg[S * kGaPad];
     const GaWhere q = ga_locate(a, blockIdx.x);
     const int E = a.E[q.l];
     const GaThread t = ga_thread<V>(a, E);
@@ -396,7 +414,7 @@ __global__ __launch_bounds__(kGaMax) void ga_bwd_stats_kernel(GaArgs a) {
     const auto load = [&](unsigned e) { return GaXD<T>{ga_load(px + e), ga_load(pd + e)}; };
     GaWalk<V, kGaUB, GaXD<T>> walk;
     walk.begin(a, q, t, load);
-    GaCoef<V, UG> k;
+    GaCoef<V, S> k;
     k.fill(a, q, t);
     float s0[V], s1[V];
     #pragma unroll
@@ -412,23 +430,28 @@ __global__ __launch_bounds__(kGaMax) void ga_bwd_stats_kernel(GaArgs a) {
                 s0[i] += g; s1[i] = __builtin_fmaf(g, xh, s1[i]);
             }
         });
-    ga_block_positions<V, float>(a, t, s0, s1, sh);
-    float* part = a.partf + ga_record(a) * a.C * 2;
-    const GaBlock blk = ga_block<V>(a);
-    for (int j = threadIdx.x; j < 2 * blk.nc; j += a.NT) {   // positions -> channels, and with gamma -> groups
-        const int c = blk.c0 + (j >> 1), k = j & 1, o0 = blk.first(c);
-        float s = 0.f;
-        for (int o = o0; o < blk.np; o += a.C) s += sh[2 * o + k];
-        part[2 * blk.c0 + j] = s;
-        if (o0 < blk.np) sh[2 * o0 + k] = s * ga_param(a.gamma, a.ptype, c, 1.f);   // (a channel's positions are read and written by this thread only)
+    #pragma unroll
+    for (int i = 0; i < V; ++i) sh[i * kGaPad + threadIdx.x] = make_float2(s0[i], s1[i]);
+    if (a.fused) {   // with gamma, for the groups
+        #pragma unroll
+        for (int i = 0; i < S; ++i) {
+            float g0 = 0.f, g1 = 0.f;
+            #pragma unroll
+            for (int m = 0; m < W; ++m) { g0 = __builtin_fmaf(k.ga[i * W + m], s0[i * W + m], g0); g1 = __builtin_fmaf(k.ga[i * W + m], s1[i * W + m], g1); }
+            shg[i * kGaPad + threadIdx.x] = make_float2(g0, g1);
+        }
     }
+    __syncthreads();
+    float2* part = reinterpret_cast<float2*>(a.partf) + ga_record(a) * a.C;
+    const GaBlock blk = ga_block<V>(a);
+    ga_bins(a.NT, blk.nc, a.R, 1, [&](int c, int r, int) {   // positions -> channels
+        float2 s = {};
+        for (int o = blk.first(blk.c0 + c); o < blk.np; o += a.C) { const float2 v = sh[(o & (V - 1)) * kGaPad + r * a.cols + o / V]; s.x += v.x; s.y += v.y; }
+        return s;
+    }, [&](int c, double c0, double c1) { part[blk.c0 + c] = make_float2((float)c0, (float)c1); });
     if (a.fused) {
-        float* gp = a.partg + ga_record(a) * a.G * 2;
-        __syncthreads();
-        ga_block_groups(a.NT, blk.ng, a.cg, [&](int g, int i, int k) {
-            const int o = blk.first((blk.g0 + g) * a.cg + i);
-            return o < blk.np ? (double)sh[2 * o + k] : 0.0;
-        }, [&](int j, double s) { gp[2 * blk.g0 + j] = (float)s; });
+        float2* gp = reinterpret_cast<float2*>(a.partg) + ga_record(a) * a.G;
+        ga_piece_groups<V, S>(a, blk, shg, [&](int g, double g0, double g1) { gp[blk.g0 + g] = make_float2((float)g0, (float)g1); });
     }
 }
 
@@ -527,9 +550,9 @@ __device__ __forceinline__ void ga_params(const GaArgs& a) {
 }
 __global__ __launch_bounds__(kGaMax) void ga_params_kernel(GaArgs a) { ga_params(a); }
 
-template <typename T, int ACT, bool UG>
+template <typename T, int ACT, int S>
 __global__ __launch_bounds__(kGaMax) void ga_bwd_apply_kernel(GaArgs a) {
-    constexpr int V = Vec16<T>::V;
+    constexpr int V = Vec16<T>::V, W = V / S;
     if ((int)blockIdx.x < a.nparam) {   // the first workgroups of a fused call: dgamma, dbeta out of all the chunks' channel sums
         if (blockIdx.y == 0) ga_params(a);
         return;
@@ -543,6 +566,8 @@ __global__ __launch_bounds__(kGaMax) void ga_bwd_apply_kernel(GaArgs a) {
     const auto load = [&](unsigned e) { return GaXD<T>{ga_stream(px + e), ga_stream(pd + e)}; };
     GaWalk<V, kGaUB, GaXD<T>> walk;
     walk.begin(a, q, t, load);
+    GaCoef<V, S> k;
+    k.fill(a, q, t);
     const float* bs = a.bstats + 2 * (size_t)(q.l * a.B + q.b) * a.G;
     if (a.fused) {   // the two means from the chunks' records
         __shared__ float sbs[2 * kGaFusedG];
@@ -553,11 +578,9 @@ __global__ __launch_bounds__(kGaMax) void ga_bwd_apply_kernel(GaArgs a) {
         __syncthreads();
         bs = sbs;
     }
-    GaCoef<V, UG> k;
-    k.fill(a, q, t);
-    float c2[UG ? 1 : V], c3[UG ? 1 : V];
+    float c2[S], c3[S];
     ga_lanes<V>(a, t, [&](int i, int, int g) {
-        if (!UG || i == 0) { c2[UG ? 0 : i] = -k.at(i).r * bs[2 * g + 1]; c3[UG ? 0 : i] = -k.at(i).r * bs[2 * g]; }
+        if (i % W == 0) { c2[i / W] = -k.at(i).r * bs[2 * g + 1]; c3[i / W] = -k.at(i).r * bs[2 * g]; }
     });
     walk.run(a, q, t, E, load,
         [&](unsigned e, int n) { return GaXD<T>{ga_load_part(px + e, n), ga_load_part(pd + e, n)}; },
@@ -567,7 +590,7 @@ __global__ __launch_bounds__(kGaMax) void ga_bwd_apply_kernel(GaArgs a) {
             #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const float xh = ga_xhat(x[i], k.at(i)), g = ga_grad<ACT>(d[i], x[i], xh, k.at(i), k.ga[i], k.be[i]);
-                d[i] = __builtin_fmaf(k.at(i).r * k.ga[i], g, __builtin_fmaf(c2[UG ? 0 : i], xh, c3[UG ? 0 : i]));
+                d[i] = __builtin_fmaf(k.at(i).r * k.ga[i], g, __builtin_fmaf(c2[i / W], xh, c3[i / W]));
             }
             ga_store_n(po + e, Vec16<T>::pack(d), n);
         });
@@ -638,11 +661,10 @@ static size_t ga_round(size_t n) { return (n + 255) & ~(size_t)255; }
 static size_t ga_chunks(const GaArgs& a) { return (size_t)a.wg0[LGD_MAX_LEVELS]; }
 static size_t ga_rows(const GaArgs& a) { return ga_chunks(a) * (size_t)(a.mixed ? a.nCB : 1); }   // records of a call
 
-template <typename T>
-static int ga_fwd(GaArgs& a, int act, hipStream_t s) {
+template <typename T, int S>
+static int ga_fwd_s(GaArgs& a, int act, hipStream_t s) {
     const dim3 grid((unsigned)ga_chunks(a), (unsigned)a.nCB);
-    if (!a.mixed && a.cg % Vec16<T>::V == 0) LGD_LAUNCH("gn_act_stats_kernel", (ga_stats_kernel<T, true>), grid, dim3((unsigned)a.NT), 0, s, a);
-    else LGD_LAUNCH("gn_act_stats_kernel", (ga_stats_kernel<T, false>), grid, dim3((unsigned)a.NT), 0, s, a);
+    LGD_LAUNCH("gn_act_stats_kernel", (ga_stats_kernel<T, S>), grid, dim3((unsigned)a.NT), 0, s, a);
     if (!a.fused) LGD_LAUNCH("gn_act_finalize_kernel", ga_finalize_kernel, dim3((unsigned)(a.L * a.B * a.G)), dim3(kGaThreads), 0, s, a);
     if (act == kActNone) LGD_LAUNCH("gn_act_apply_kernel", (ga_apply_kernel<T, kActNone>), grid, dim3((unsigned)a.NT), 0, s, a);
     else if (act == kActRelu) LGD_LAUNCH("gn_act_apply_kernel", (ga_apply_kernel<T, kActRelu>), grid, dim3((unsigned)a.NT), 0, s, a);
@@ -650,31 +672,46 @@ static int ga_fwd(GaArgs& a, int act, hipStream_t s) {
     return check_launch();
 }
 
-template <typename T, int ACT, bool UG>
+// f(pieces of a vector)
+template <typename T, typename F>
+static int ga_pieces(const GaArgs& a, F f) {
+    constexpr int V = Vec16<T>::V;
+    const int S = V / ga_gcd(a.cg, V);
+    if (S == 1) return f(std::integral_constant<int, 1>());
+    if (S == 2) return f(std::integral_constant<int, 2>());
+    if constexpr (V == 8) if (S == 4) return f(std::integral_constant<int, 4>());
+    return f(std::integral_constant<int, V>());
+}
+template <typename T>
+static int ga_fwd(GaArgs& a, int act, hipStream_t s) {
+    return ga_pieces<T>(a, [&](auto S) { return ga_fwd_s<T, decltype(S)::value>(a, act, s); });
+}
+
+template <typename T, int ACT, int S>
 static int ga_bwd(GaArgs& a, hipStream_t s) {
     const dim3 grid((unsigned)ga_chunks(a), (unsigned)a.nCB);
-    LGD_LAUNCH("gn_act_bwd_stats_kernel", (ga_bwd_stats_kernel<T, ACT, UG>), grid, dim3((unsigned)a.NT), 0, s, a);
+    LGD_LAUNCH("gn_act_bwd_stats_kernel", (ga_bwd_stats_kernel<T, ACT, S>), grid, dim3((unsigned)a.NT), 0, s, a);
     const bool params = a.dgamma || a.dbeta;
     if (a.fused) {
         const unsigned np = params ? (unsigned)((a.C + kGaParamC - 1) / kGaParamC) : 0u;
         a.nparam = (int)np;
-        if (a.out[0]) LGD_LAUNCH("gn_act_bwd_apply_kernel", (ga_bwd_apply_kernel<T, ACT, UG>), dim3(grid.x + np, grid.y), dim3((unsigned)a.NT), 0, s, a);
+        if (a.out[0]) LGD_LAUNCH("gn_act_bwd_apply_kernel", (ga_bwd_apply_kernel<T, ACT, S>), dim3(grid.x + np, grid.y), dim3((unsigned)a.NT), 0, s, a);
         else if (params) LGD_LAUNCH("gn_act_bwd_param_kernel", ga_params_kernel, dim3(np), dim3((unsigned)a.NT), 0, s, a);
         return check_launch();
     }
     LGD_LAUNCH("gn_act_bwd_finalize_kernel", ga_bwd_finalize_kernel, dim3((unsigned)(a.L * a.B * a.G)), dim3(256), 0, s, a);
     if (params) LGD_LAUNCH("gn_act_bwd_param_kernel", ga_param_kernel, dim3((unsigned)((a.C + 63) / 64)), dim3(256), 0, s, a);
-    if (a.out[0]) LGD_LAUNCH("gn_act_bwd_apply_kernel", (ga_bwd_apply_kernel<T, ACT, UG>), grid, dim3((unsigned)a.NT), 0, s, a);
+    if (a.out[0]) LGD_LAUNCH("gn_act_bwd_apply_kernel", (ga_bwd_apply_kernel<T, ACT, S>), grid, dim3((unsigned)a.NT), 0, s, a);
     return check_launch();
 }
-template <typename T, bool UG>
-static int ga_bwd_act(GaArgs& a, int act, hipStream_t s) {
-    if (act == kActNone) return ga_bwd<T, kActNone, UG>(a, s);
-    if (act == kActRelu) return ga_bwd<T, kActRelu, UG>(a, s);
-    return ga_bwd<T, kActSilu, UG>(a, s);
-}
 template <typename T>
-static int ga_bwd_ug(GaArgs& a, int act, hipStream_t s) { return a.cg % Vec16<T>::V ? ga_bwd_act<T, false>(a, act, s) : ga_bwd_act<T, true>(a, act, s); }
+static int ga_bwd_any(GaArgs& a, int act, hipStream_t s) {
+    return ga_pieces<T>(a, [&](auto S) {
+        if (act == kActNone) return ga_bwd<T, kActNone, decltype(S)::value>(a, s);
+        if (act == kActRelu) return ga_bwd<T, kActRelu, decltype(S)::value>(a, s);
+        return ga_bwd<T, kActSilu, decltype(S)::value>(a, s);
+    });
+}
 
 }  // namespace lgd
 
@@ -739,9 +776,9 @@ int lgd_gn_act_bwd(const void* const* x_host, const void* const* dy_host, const 
     a.bstats = reinterpret_cast<float*>(w);
     w += lgd::ga_round((size_t)L * B * G * 2 * sizeof(float));
     a.partg = reinterpret_cast<float*>(w);
-    if (dtype == LGD_F32) return lgd::ga_bwd_ug<float>(a, act, s);
-    if (dtype == LGD_BF16) return lgd::ga_bwd_ug<__bf16>(a, act, s);
-    return lgd::ga_bwd_ug<_Float16>(a, act, s);
+    if (dtype == LGD_F32) return lgd::ga_bwd_any<float>(a, act, s);
+    if (dtype == LGD_BF16) return lgd::ga_bwd_any<__bf16>(a, act, s);
+    return lgd::ga_bwd_any<_Float16>(a, act, s);
 }
 
 }  // extern "C"

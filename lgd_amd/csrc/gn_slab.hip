@@ -142,6 +142,12 @@ __global__ __launch_bounds__(kSlabThreads) void slab_fwd_kernel(SlabArgs a) {
             if (u < mine) x[u] = slab_load<T, VW>(px + e);
         }
     }
+    int c[E];
+    uint32_t wga[E] = {}, wbe[E] = {};   // (asked for in front of the barriers)
+    #pragma unroll
+    for (int i = 0; i < E; ++i) c[i] = mine ? c0 + i : 0;
+    ga_param_words<E>(a.gamma, a.ptype, c, wga);
+    ga_param_words<E>(a.beta, a.ptype, c, wbe);
     int lg[MULTI ? E : 1];   // the lanes' groups in the slab
     if constexpr (MULTI) {
         #pragma unroll
@@ -180,10 +186,12 @@ __global__ __launch_bounds__(kSlabThreads) void slab_fwd_kernel(SlabArgs a) {
         } else { mu[0] = m; r[0] = rs; }
     }
     double A[E], Bc[E];   // z = x (r gamma) + (beta - mu r gamma), one fp64 FMA
-    #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        A[i] = r[MULTI ? i : 0] * (double)(mine ? ga_param(a.gamma, a.ptype, c0 + i, 1.f) : 0.f);
-        Bc[i] = fma(-mu[MULTI ? i : 0], A[i], (double)(mine ? ga_param(a.beta, a.ptype, c0 + i, 0.f) : 0.f));
+    {
+        float ga[E], be[E];
+        ga_param_values<E>(a.gamma, a.ptype, wga, 1.f, ga);
+        ga_param_values<E>(a.beta, a.ptype, wbe, 0.f, be);
+        #pragma unroll
+        for (int i = 0; i < E; ++i) { A[i] = r[MULTI ? i : 0] * (double)ga[i]; Bc[i] = fma(-mu[MULTI ? i : 0], A[i], (double)be[i]); }
     }
     unsigned e = ((unsigned)row0 * a.C + c0) * (unsigned)sizeof(T);
     slab_forget(x);
@@ -250,12 +258,23 @@ __device__ __forceinline__ void slab_bwd_body(const SlabArgs& a, const SlabWhere
         }
     }
     SlabLanes<E, MULTI> k;
-    const double* st = a.stats + 2 * ((size_t)lb * a.G + q.sl * a.ng);
-    if constexpr (!MULTI) k.grp[0] = ga_group(st, 0);
-    #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        if constexpr (MULTI) { k.lg[i] = mine ? (col * E + i) / a.cg : 0; k.grp[i] = ga_group(st, k.lg[i]); }
-        k.ga[i] = mine ? ga_param(a.gamma, a.ptype, c0 + i, 1.f) : 0.f; k.be[i] = mine ? ga_param(a.beta, a.ptype, c0 + i, 0.f) : 0.f;
+    const double2* st = reinterpret_cast<const double2*>(a.stats) + (size_t)lb * a.G + q.sl * a.ng;
+    {
+        double2 m[MULTI ? E : 1];
+        int c[E];
+        #pragma unroll
+        for (int i = 0; i < E; ++i) {
+            c[i] = mine ? c0 + i : 0;
+            if constexpr (MULTI) { k.lg[i] = mine ? (col * E + i) / a.cg : 0; m[i] = st[k.lg[i]]; }
+        }
+        if constexpr (!MULTI) m[0] = st[0];
+        uint32_t wga[E] = {}, wbe[E] = {};
+        ga_param_words<E>(a.gamma, a.ptype, c, wga);
+        ga_param_words<E>(a.beta, a.ptype, c, wbe);
+        ga_param_values<E>(a.gamma, a.ptype, wga, 1.f, k.ga);
+        ga_param_values<E>(a.beta, a.ptype, wbe, 0.f, k.be);
+        #pragma unroll
+        for (int i = 0; i < (MULTI ? E : 1); ++i) k.grp[i] = ga_group(m[i].x, m[i].y);
     }
     float s0[E] = {}, s1[E] = {};
     #pragma unroll
