@@ -370,13 +370,14 @@ static bool slab_plan(SlabArgs& a, SlabPlan& p, const GaCall& c) {
     p.VW = row % 16 == 0 ? 4 : row % 8 == 0 ? 2 : 1;
     if (ng > 1 && size == 2 && p.VW == 4) p.VW = 2;   // a group for each of 8 lanes does not fit the registers
     // One workgroup does all of a slab's arithmetic on one CU, the streaming kernels spread it over the chip at the price of a second read and a second
-    // launch: what decides is the number of elements on the busiest CU.  Measured on 110 shapes, B 1 - 16, 144 - 1280 channels, 16^2 - 64^2 pixels (us, this
-    // kernel / streaming, forward and backward):  2 - 5 K elements 5.3 / 13, 8 / 17;  20 K 9.4 / 16.5, 18 / 25;  41 K 20 / 18, 33 / 30;  66 K 32 / 26, 60 / 40.
-    // Rows that only dwords divide cost twice the accesses (41 K: 24 / 15), rows under 16 bytes more of the lines' traffic (16 K at 4 bytes: 16 / 11).
+    // launch: what decides is the number of elements on the busiest CU.  Measured on 150 shapes, B 1 - 16, 33 - 1280 channels, 8^2 - 64^2 pixels (us, this
+    // kernel / streaming, forward and backward):  2 K elements 4.7 / 9.8, 7.9 / 13.3;  8 K 5.3 / 9.9, 9.9 / 13.4;  18 K 8.7 / 12.7, 19.8 / 20.6;  33 K 9.9 /
+    // 10.7, 19.2 / 14.9.  Rows under 16 bytes cost more of the lines' traffic (18 K at 4 bytes 17 / 11), rows of under 8 elements that only dwords divide
+    // twice the accesses as well (5 fp32 channels, 20 K: 20 / 12; 11 of them, 18 K: 10.9 / 11.9), several groups their sums one by one (33 K: 11.4 / 10.1)
     long long total = 0;
     for (int l = 0; l < c.L; ++l) total += (long long)c.hw[2 * l] * c.hw[2 * l + 1] * c.B * c.C;
     const long long slab = (long long)most * ng * cg, cu = slab > total / 256 ? slab : total / 256;
-    if (cu > 24576LL * (row < 16 ? row : 16) / 16 / (p.VW == 1 ? 2 : 1) / (ng > 1 ? 2 : 1)) return false;   // (several groups: 16 K 16 / 11)
+    if (cu > 24576LL * (row < 16 ? row : 16) / 16 / (p.VW == 1 && row < 8 * size ? 2 : 1) / (ng > 1 ? 2 : 1)) return false;
     a = SlabArgs{};
     a.VR = row / (4 * p.VW);
     if (a.VR > kSlabThreads || ng * cg > kSlabCh || (long long)most * c.C * size >= (1LL << 32)) return false;   // (32-bit offsets in a sample)
