@@ -160,10 +160,13 @@ __device__ __forceinline__ void ga_lanes(const GaArgs& a, const GaThread& t, F f
 template <typename T> struct GaX { lgd_u32x4 x; };
 template <typename T> struct GaXD { lgd_u32x4 x, d; };
 
-template <typename T> __device__ __forceinline__ lgd_u32x4 ga_load_part(const T* p, int count) {   // count < V elements, the rest zero
+// count (1 .. V - 1) elements, the rest zero: all loads at once, those behind the end from the last element (branches around them wait for each other, 5 us)
+template <typename T> __device__ __forceinline__ lgd_u32x4 ga_load_part(const T* p, int count) {
     T tmp[Vec16<T>::V];
     #pragma unroll
-    for (int i = 0; i < Vec16<T>::V; ++i) tmp[i] = i < count ? p[i] : (T)0.f;
+    for (int i = 0; i < Vec16<T>::V; ++i) tmp[i] = p[i < count ? i : count - 1];
+    #pragma unroll
+    for (int i = 0; i < Vec16<T>::V; ++i) tmp[i] = i < count ? tmp[i] : (T)0.f;
     lgd_u32x4 u;
     __builtin_memcpy(&u, tmp, 16);
     return u;
@@ -302,7 +305,7 @@ __global__ __launch_bounds__(kGaThreads) void ga_finalize_kernel(GaArgs a) {
 // slices meet in LDS, in a fixed order.  P2: pair of the records.  Barriers inside
 template <typename P2, typename Put>
 __device__ __forceinline__ void ga_records(int nt, const P2* __restrict__ p, int K, int G, const GaBlock& blk, Put put) {
-    __shared__ double tmp[kGaMax][2];
+    __shared__ double2 tmp[kGaMax];
     int sub = 1;
     while (sub < blk.ng && 2 * sub <= nt) sub <<= 1;
     const int slices = nt / sub, sl = threadIdx.x / sub;
@@ -319,13 +322,19 @@ __device__ __forceinline__ void ga_records(int nt, const P2* __restrict__ p, int
                 for (int u = 0; u < kGaRecordsU; ++u) { s0 += (double)v[u].x; s1 += (double)v[u].y; }
             }
         }
-        if (slices > 1) {
-            tmp[threadIdx.x][0] = s0; tmp[threadIdx.x][1] = s1;
+        if (slices > 1) tmp[threadIdx.x] = make_double2(s0, s1);
+        for (int m = slices; m > 1;) {   // eight at a time
+            const int next = (m + 7) >> 3;
             __syncthreads();
-            if (sl == 0) for (int i = 1; i < slices; ++i) { s0 += tmp[threadIdx.x + i * sub][0]; s1 += tmp[threadIdx.x + i * sub][1]; }
+            if (sl < next) {
+                s0 = s1 = 0.0;
+                for (int i = sl; i < m; i += next) { const double2 v = tmp[threadIdx.x + (i - sl) * sub]; s0 += v.x; s1 += v.y; }
+            }
+            m = next;
+            __syncthreads();
+            if (m > 1 && sl < m) tmp[threadIdx.x] = make_double2(s0, s1);
         }
         if (sl == 0 && g < gend) put(g, s0, s1);
-        if (slices > 1) __syncthreads();
     }
 }
 
