@@ -651,8 +651,10 @@ int lgd_sgd_norm_step_host(const lgd_sgd_tensor* table_host, const int32_t* blk_
 /* ------------------------------------------------------------------ GroupNorm + activation, channels last
  * GroupNorm(G, per-channel affine) then act over L maps stored (B, H_l, W_l, C), one module for all of them; dtype LGD_F32 / LGD_BF16 /
  * LGD_F16 for x, y, dy, dx; gamma / beta (C entries, either may be NULL = 1 / 0) and their gradients in param_dtype.
- * act: LGD_ACT_NONE, LGD_ACT_RELU, LGD_ACT_SILU.  All pointers aligned to the element (16 bytes is fastest); H_l * W_l * C below 2^31.
- *   stats: fp64 [L*B*G][2] (mean, 1/sqrt(var + eps)), 16-byte aligned, written by fwd, read by bwd;  ws: lgd_gn_act_ws_bytes(..., backward) bytes, 16-byte aligned
+ * act: LGD_ACT_NONE, LGD_ACT_RELU, LGD_ACT_SILU.  All pointers aligned to the element (16 bytes is fastest); H_l * W_l * C below 2^31,
+ * L * B * G below 2^30.
+ *   stats: fp64 [L*B*G][2] (mean, 1/sqrt(var + eps)), 16-byte aligned, written by fwd, read by bwd;  ws: lgd_gn_act_ws_bytes(..., backward) bytes,
+ *   16-byte aligned
  *   (0: none is needed, ws may be NULL; (size_t)-1: not a call these entries take)
  * backward: dx_host NULL: no input gradients; dgamma / dbeta NULL: not wanted.  Sums run in a fixed order (no atomics).
  */

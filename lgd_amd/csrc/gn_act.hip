@@ -12,15 +12,15 @@
 //
 // Precision.  Sums of x and x^2 are fp64 (gfx950 runs fp64 FMA at the rate of unpacked fp32), the statistics stay fp64, and z = x (r gamma) +
 // (beta - mu r gamma) is ONE fp64 FMA per element: the sign a ReLU's gradient hangs on is decided in 64 bits.  Sums of the backward are fp32 over one
-// thread's rows of a chunk (<= a few hundred terms) and its workgroup, fp64 from there on.  Outputs are rounded once (fp32 -> 16 bits).
+// thread's rows of a chunk (<= a few hundred terms), fp64 across its workgroup, one fp32 word per chunk, fp64 across those.  Outputs are rounded once (fp32 -> 16 bits).
 #include "gn_act.h"
 
 #include <type_traits>
 
 namespace lgd {
 
-// Workgroups of a streaming call, about: two for every CU, in step.  8 x 320 x 256 x 256 bf16, forward / backward us: 512 168 / 291, 768 197 / 345 (three on
-// some CUs, four on others), 1024 177 / 299
+// Workgroups of a streaming call, about: two for every CU, in step.  8 x 320 x 256 x 256 bf16, forward / backward us: 512 168 / 290 (5.1 TB/s of
+// what they move), 768 197 / 345 (three on some CUs, four on others), 1024 177 / 299
 constexpr int kGaWorkgroups = 512;
 constexpr int kGaU = 4, kGaUB = 2;     // vectors (of x; of x and dy each) of a thread in flight
 constexpr int kGaRecordsU = 8;         // records of a thread in flight

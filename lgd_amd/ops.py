@@ -349,6 +349,7 @@ def group_norm_act(xs, groups, weight=None, bias=None, act="relu", eps=1e-5):
     them (group_norm_relu is the NCHW fp32 form): act "none", "relu" or "silu"; weight / bias (C,) fp32, bf16 or fp16, or None.  Maps that are
     not dense in torch.channels_last order are copied into it; the outputs and the input gradients are channels-last, in the maps' type,
     rounded once (statistics and the sign under a ReLU are 64-bit).  A map without elements gives one without elements.  First derivatives only.
+    A backward captured into a graph takes leaves that no older graph from another stream holds (refused otherwise).
     The checks, the allocations and the autograd node are csrc/host.cpp: on small maps they are most of what a call costs."""
     code = _GN_ACTS.get(act)
     if code is None:
