@@ -143,6 +143,23 @@ def test_group_norm_act_many_groups(shape, dtype):
     assert torch.equal(gw, dw) and torch.equal(gb, db)
 
 
+@pytest.mark.parametrize("seed", range(60))
+def test_group_norm_act_over_the_range(seed):
+    """drawn shapes: batches, groups of 1 to 325 channels, one to sixteen maps of any sides, every type, parameters of another type"""
+    import random
+    r = random.Random(seed)
+    G, B, L = r.choice([1, 2, 3, 5, 7, 8, 11, 16, 32, 33, 64]), r.choice([1, 1, 2, 3, 9]), r.choice([1, 1, 2, 3, 5, 16])
+    C = G * r.choice([1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 16, 17, 20, 24, 31, 40, 64, 80, 325])
+    side = max(1, int((2e6 / (B * C * L)) ** 0.5))
+    hws = [(max(1, int(side * r.uniform(0.2, 2))), max(1, int(side * r.random()))) for _ in range(L)]
+    dtype, act, ptype = r.choice(list(TYPES)), r.choice(["none", "relu", "silu"]), r.choice(list(TYPES))
+    T = TYPES[dtype]
+    xs, dys = _maps(B, C, hws, T, 1000 * seed, r.choice([0.1, 1.0, 3.0]), r.choice([0.0, 0.5, -20.0])), _maps(B, C, hws, T, 1000 * seed + 500)
+    w, b = _params(C, TYPES[ptype], 7 * seed)
+    ys, dxs, dw, db = _run(xs, G, w, b, act, 1e-5, dys)
+    _check(xs, G, w, b, act, 1e-5, dys, ys, dxs, dw, db)
+
+
 @pytest.mark.parametrize("weight,bias,ptype", [(True, False, "fp32"), (False, True, "bf16"), (False, False, "fp32"), (True, True, "fp16"), (True, True, "fp32")])
 def test_group_norm_act_parameters(weight, bias, ptype):
     """either parameter may be missing, and theirs may be another type than the maps'"""
