@@ -184,12 +184,9 @@ struct GnBackward : public Node {
         }
         if (again) {
             torch::autograd::edge_list edges;
-            auto edge = [&](const Tensor& t) {
+            for (const auto& e : next_edges()) if (e.is_valid()) edges.push_back(e);   // the call's own inputs: what is saved may be a copy of them
+            for (const Tensor& t : dys)
                 if (t.defined() && t.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(t));
-            };
-            for (const Tensor& t : xs) edge(t);
-            edge(wv); edge(bv);
-            for (const Tensor& t : dys) edge(t);
             if (!edges.empty()) {
                 auto node = std::shared_ptr<GnNoSecond>(new GnNoSecond(), torch::autograd::deleteNode);
                 node->set_next_edges(std::move(edges));
