@@ -511,16 +511,40 @@ PyObject* py_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// sgd_step(parameters, momentum buffers, plan, [lr, weight decay, momentum] of every set, norm code or None, clip) -> the norms (by value: True);
-// None: the parameters that have a gradient are not the plan's; False: they are not on a GPU.  Lists of tensors (None where a parameter has no row);
-// plan: six bytes objects in the order of SgdPlan
+// do the optimizers' states still hold what the plan was made with?  held: parameter, its state, its momentum buffer (or None), entry by entry; compared
+// as objects.  1 yes, 0 no, -1 an error is set
+int state_held(PyObject* states, PyObject* held) {
+    static PyObject* const key = PyUnicode_InternFromString("momentum_buffer");
+    const Py_ssize_t n = PyList_GET_SIZE(held);
+    Py_ssize_t k = 0;
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(states); ++i) {
+        PyObject* state = PyList_GET_ITEM(states, i);
+        if (!PyDict_Check(state)) { PyErr_SetString(PyExc_TypeError, "an optimizer's state must be a dict"); return -1; }
+        PyObject *p, *entry;
+        for (Py_ssize_t at = 0; PyDict_Next(state, &at, &p, &entry); k += 3) {
+            if (k + 3 > n || PyList_GET_ITEM(held, k) != p || PyList_GET_ITEM(held, k + 1) != entry) return 0;
+            if (!PyDict_Check(entry)) { PyErr_SetString(PyExc_TypeError, "a parameter's optimizer state must be a dict"); return -1; }
+            PyObject* m = PyDict_GetItemWithError(entry, key);
+            if (!m && PyErr_Occurred()) return -1;
+            if (PyList_GET_ITEM(held, k + 2) != (m ? m : Py_None)) return 0;
+        }
+    }
+    return k == n;
+}
+
+// sgd_step(parameters, momentum buffers, plan, [lr, weight decay, momentum] of every set, norm code or None, clip, the optimizers' states, what they held
+// when the plan was made) -> the norms (by value: True); None: the parameters that have a gradient, or the states, are not the plan's; False: they are
+// not on a GPU.  Lists of tensors (None where a parameter has no row); plan: six bytes objects in the order of SgdPlan
 PyObject* py_sgd_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 6 || !PyList_Check(a[0]) || !PyList_Check(a[1]) || PyList_GET_SIZE(a[0]) != PyList_GET_SIZE(a[1]) || !PyTuple_Check(a[2]) ||
-        PyTuple_GET_SIZE(a[2]) != 6 || !PyList_Check(a[3])) {
-        PyErr_SetString(PyExc_TypeError, "sgd_step(list, list, plan, list, norm code, clip)");
+    if (n != 8 || !PyList_Check(a[0]) || !PyList_Check(a[1]) || PyList_GET_SIZE(a[0]) != PyList_GET_SIZE(a[1]) || !PyTuple_Check(a[2]) ||
+        PyTuple_GET_SIZE(a[2]) != 6 || !PyList_Check(a[3]) || !PyList_Check(a[6]) || !PyList_Check(a[7])) {
+        PyErr_SetString(PyExc_TypeError, "sgd_step(list, list, plan, list, norm code, clip, list, list)");
         return nullptr;
     }
+    const int same = state_held(a[6], a[7]);
+    if (same < 0) return nullptr;
+    if (!same) Py_RETURN_NONE;
     const void* part[6];
     Py_ssize_t size[6];
     for (int i = 0; i < 6; ++i) {

@@ -107,7 +107,6 @@ class FusedClipSGD:
                 raise hip.LgdHipError("clipping by norm takes 1 to 16 optimizers (LGD_MAX_SGD_GROUPS) that share no parameter")
         self._numel = np.array([p.numel() for p in self.params], dtype=np.int64)
         self._m_ref = [None] * n   # momentum buffers
-        self._state_ids = None     # Optimizer.load_state_dict installs a new state dict: the cached buffers are then stale
         self._grp = np.array([k * 4096 + gi for k, gi in self.owner], dtype=np.int64)
         self._plan = None
 
@@ -117,27 +116,25 @@ class FusedClipSGD:
             p.grad = None
 
     def _buffers(self, idx):
-        """momentum buffers of the parameters `idx` (created zero-filled on first use: torch's first step sets buf = d_p, which
-        is what mu * 0 + d_p gives); the cache is dropped when an optimizer's state dict has been replaced (load_state_dict)."""
-        ids = [id(o.state) for o in self.optimizers]
-        if ids != self._state_ids:
-            self._state_ids = ids
-            self._m_ref = [None] * len(self.params)
+        """momentum buffers of the parameters `idx` as the optimizers hold them now (created zero-filled on first use: torch's first
+        step sets buf = d_p, which is what mu * 0 + d_p gives)."""
         for i in idx:
-            if self._m_ref[i] is not None:
-                continue
             p = self.params[i]
             st = self.optimizers[self.owner[i][0]].state[p]
             m = st.get("momentum_buffer")
             if m is None:
                 m = st["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
+            elif m is self._m_ref[i]:
+                continue
             if not (m.is_cuda and m.dtype == torch.float32 and m.is_contiguous() and m.numel() == p.numel()):
                 raise hip.LgdHipError("momentum buffer of a fused-SGD parameter must be a dense fp32 device tensor")
             self._m_ref[i] = m
 
     def _make_plan(self):
-        """(parameter groups whose hyper-parameters the table needs, the columns of csrc/host.cpp's SgdPlan): what follows from the set of
-        parameters that have a gradient; None where none has"""
+        """(parameter groups whose hyper-parameters the table needs, the columns of csrc/host.cpp's SgdPlan, what the optimizers' states held):
+        what follows from the set of parameters that have a gradient; None where none has.  The states' entries (parameter, its state, its
+        momentum buffer) are kept as objects, so that none of their addresses can come back as another's while the plan lives: a state dict that
+        load_state_dict put in, a buffer that was replaced or an entry that was dropped is seen at the next step"""
         idx = [i for i, p in enumerate(self.params) if p.grad is not None]
         if not idx:
             return None
@@ -152,7 +149,8 @@ class FusedClipSGD:
         tab["reserved"] = owner = self._grp[ii] // 4096   # clipping by norm: the row's optimizer
         border = np.searchsorted(owner, np.arange(len(self.optimizers) + 1))   # the table is ordered by optimizer
         columns = (ii.astype(np.int32), tab, blk, which.astype(np.int32), border.astype(np.int32), blk[border])
-        return [divmod(key, 4096) for key in keys.tolist()], tuple(c.tobytes() for c in columns)
+        held = [x for o in self.optimizers for p, st in o.state.items() for x in (p, st, st.get("momentum_buffer"))]
+        return [divmod(key, 4096) for key in keys.tolist()], tuple(c.tobytes() for c in columns), held
 
     @torch.no_grad()
     def step(self):
@@ -160,20 +158,18 @@ class FusedClipSGD:
         if by_norm and not float(self.clip_norm) >= 0:
             raise hip.LgdHipError("clip_norm must not be negative, got %r" % (self.clip_norm,))
         code, clip = (_norm_code(self.norm_type), float(self.clip_norm)) if by_norm else (None, self.clip_value)
-        if self._plan is not None and [id(o.state) for o in self.optimizers] != self._state_ids:
-            self._plan = None
         got = None
-        while got is None:   # a plan serves until another set of parameters has gradients
+        while got is None:   # a plan serves until another set of parameters has gradients or a state holds something else
             if self._plan is None:
                 self._plan = self._make_plan()
                 if self._plan is None:
                     if by_norm:
                         self.total_norms = torch.zeros(len(self.optimizers), device=self.params[0].device if self.params else None)
                     return
-            keys, columns = self._plan
+            keys, columns, held = self._plan
             groups = [self.optimizers[o].param_groups[j] for o, j in keys]
             hyper = [float(g[name]) for g in groups for name in ("lr", "weight_decay", "momentum")]
-            got = hip.host().sgd_step(self.params, self._m_ref, columns, hyper, code, clip)
+            got = hip.host().sgd_step(self.params, self._m_ref, columns, hyper, code, clip, [o.state for o in self.optimizers], held)
             if got is None:
                 self._plan = None
         if got is False:

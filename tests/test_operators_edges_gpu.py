@@ -1,4 +1,6 @@
-"""Calls of the channels-last GroupNorm, the gradient norms and the fused SGD step at their edges: differentiating again."""
+"""Calls of the channels-last GroupNorm, the gradient norms and the fused SGD step at their edges: differentiating again, optimizer states that come and go."""
+import copy
+
 import pytest
 import torch
 
@@ -64,3 +66,65 @@ def test_a_derivative_by_the_output_gradient_raises(form):
     g, = torch.autograd.grad(ops.group_norm_act([x], 2)[0], [x], dy, create_graph=True)
     with pytest.raises(RuntimeError, match="second derivative"):
         torch.autograd.grad(g.square().sum(), [dy])
+
+
+def _sgd(count, seed=7):
+    g = torch.Generator().manual_seed(seed)
+    ps = [torch.nn.Parameter(torch.randn(5 + 3 * i, generator=g).to(DEV)) for i in range(count)]
+    return ps, [torch.optim.SGD(ps[:2], 0.1, momentum=0.9), torch.optim.SGD(ps[2:], 0.2, momentum=0.8, weight_decay=1e-3)]
+
+
+def _load(optimizers, factor, times):
+    for o in optimizers:
+        for k in range(times):
+            sd = copy.deepcopy(o.state_dict())
+            for st in sd["state"].values():
+                st["momentum_buffer"] = st["momentum_buffer"] * factor + 1.0
+            o.load_state_dict(sd)
+
+
+def _replace(optimizers):
+    for o in optimizers:
+        for st in o.state.values():
+            st["momentum_buffer"] = st["momentum_buffer"] * -2.0
+
+
+def _drop(optimizers):
+    for o in optimizers:
+        o.state.clear()
+
+
+def _forget(optimizers):   # the key leaves the inner dict: both sides begin again at zero
+    for o in optimizers:
+        for st in o.state.values():
+            st.pop("momentum_buffer")
+
+
+CHANGES = {"load": lambda o: _load(o, -1.5, 1), "load twice": lambda o: _load(o, -1.5, 2), "load four times": lambda o: _load(o, 0.5, 4),
+           "replaced buffers": _replace, "cleared": _drop, "one optimizer": lambda o: _load(o[1:], 2.0, 2), "forgotten": _forget}
+
+
+@pytest.mark.parametrize("limit", [None, 0.5])
+@pytest.mark.parametrize("count", [6, 90])
+@pytest.mark.parametrize("change", list(CHANGES))
+def test_the_step_follows_the_optimizers_state(change, count, limit):
+    """momentum that is loaded, replaced or dropped between two steps counts in the next one, and the optimizers hold what the step wrote.  Tolerance: torch's own
+    step rounds each operation and its norm is fp32; 2e-5 of the value covers a few steps of that (2^-24 each), 2e-6 the cancelled ones"""
+    from lgd_amd import optim
+    (pa, oa), (pb, ob) = _sgd(count), _sgd(count)
+    fused = optim.FusedClipSGD(ob, clip_norm=limit)
+    for step in range(4):
+        for i, (a, b) in enumerate(zip(pa, pb)):
+            a.grad = _rand(tuple(a.shape), 100 * step + i)
+            b.grad = a.grad.clone()
+        for o in oa:
+            if limit is not None:
+                torch.nn.utils.clip_grad_norm_([p for g in o.param_groups for p in g["params"]], limit)
+            o.step()
+        fused.step()
+        for a, b, k in zip(pa, pb, [0, 0] + [1] * count):
+            assert torch.allclose(a, b, rtol=2e-5, atol=2e-6), (step, k)
+            assert torch.allclose(oa[k].state[a]["momentum_buffer"], ob[k].state[b]["momentum_buffer"], rtol=2e-5, atol=2e-6), (step, k)
+        if step in (0, 2):
+            CHANGES[change](oa)
+            CHANGES[change](ob)
