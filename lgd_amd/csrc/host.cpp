@@ -384,8 +384,11 @@ Sgd sgd_step(PyObject* params, PyObject* momenta, const SgdPlan& plan, const std
     memcpy(t, plan.table, (size_t)k * sizeof(lgd_sgd_tensor));
     Runs runs;
     for (int j = 0; j < k; ++j) {
-        if (!dense_f32(gs[j]) || gs[j].device() != dev) refuse("fused SGD needs dense contiguous fp32 gradients on one device");
-        if (!dense_f32(ps[j])) refuse("fused SGD needs dense contiguous fp32 parameters");
+        // (the sizes of parameters and momenta are checked against the plan's by the caller; `.data` can be anything by now)
+        if (!dense_f32(gs[j]) || gs[j].device() != dev || gs[j].numel() != t[j].n)
+            refuse("fused SGD needs dense contiguous fp32 gradients of their parameters' sizes on one device");
+        if (!dense_f32(ps[j]) || ps[j].device() != dev) refuse("fused SGD needs dense contiguous fp32 parameters, beside their gradients");
+        if (!dense_f32(ms[j]) || ms[j].device() != dev) refuse("fused SGD needs dense contiguous fp32 momentum buffers, beside their gradients");
         t[j].p = ps[j].data_ptr<float>(); t[j].g = gs[j].data_ptr<float>(); t[j].m = ms[j].data_ptr<float>();
         const float* h = &hyper[3 * (size_t)plan.set[j]];
         t[j].lr = h[0]; t[j].wd = h[1]; t[j].mu = h[2];

@@ -128,3 +128,23 @@ def test_the_step_follows_the_optimizers_state(change, count, limit):
         if step in (0, 2):
             CHANGES[change](oa)
             CHANGES[change](ob)
+
+
+@pytest.mark.parametrize("limit", [None, 0.5])
+def test_the_step_refuses_tensors_that_no_longer_fit(limit):
+    """`.data` of a momentum buffer, a parameter or a gradient replaced by another type, device, order or size between two steps: refused, nothing is changed"""
+    from lgd_amd import hip, optim
+    for what, other in [("m", lambda t: t.half()), ("m", lambda t: t.cpu()), ("m", lambda t: torch.zeros(2 * t.numel(), device=DEV)[::2]),
+                        ("g", lambda t: torch.ones(3, device=DEV)), ("g", lambda t: torch.ones(2 * t.numel(), device=DEV)),
+                        ("g", lambda t: t.half()), ("p", lambda t: t.half()), ("p", lambda t: t.cpu())]:
+        ps, opts = _sgd(4)
+        fused = optim.FusedClipSGD(opts, clip_norm=limit)
+        for p in ps:
+            p.grad = torch.ones_like(p)
+        fused.step()
+        t = {"m": opts[1].state[ps[2]]["momentum_buffer"], "g": ps[2].grad, "p": ps[2]}[what]
+        t.data = other(t.data)
+        before = [p.detach().clone() for p in ps]
+        with pytest.raises(hip.LgdHipError, match="fused SGD needs"):
+            fused.step()
+        assert all(torch.equal(p, b) for p, b in zip(ps, before)), what
