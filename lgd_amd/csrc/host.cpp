@@ -372,7 +372,8 @@ Sgd sgd_step(PyObject* params, PyObject* momenta, const SgdPlan& plan, const std
     const c10::Device dev = gs[0].device();
     if (!dev.is_cuda()) return Sgd::kNotGpu;
     const c10::DeviceGuard guard(dev);
-    if (by_norm && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
+    // (a replay would upload whatever the pinned block holds by then: addresses of nothing)
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
         refuse("the fused step's table (addresses, learning rates) is the host's of this call: it cannot be captured into a graph");
     at::AutoDispatchBelowADInplaceOrView below;
     const int64_t bytes = (int64_t)k * sizeof(lgd_sgd_tensor) + 4 * (k + 1), room = (bytes + 15) / 16 * 16;

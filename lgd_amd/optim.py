@@ -86,7 +86,8 @@ class FusedClipSGD:
     """step() = clip + update of every parameter that has a gradient, over all the given torch.optim.SGD objects.
     clip_value: element-wise clamp.  clip_norm: the gradients of EACH optimizer are scaled by min(1, clip_norm / (norm + 1e-6)) of their own
     norm (norm_type 2, 1 or inf) -- torch.nn.utils.clip_grad_norm_ per optimizer, then its step(); `total_norms` then holds the norms
-    before clipping of the last step (one fp32 per optimizer, on the device).  Neither: no clipping.  The clipped gradients are written back."""
+    before clipping of the last step (one fp32 per optimizer, on the device).  Neither: no clipping.  The clipped gradients are written back.
+    A step cannot be captured into a graph (refused): its table of addresses and learning rates is the host's of that call."""
 
     def __init__(self, optimizers, clip_value=None, clip_norm=None, norm_type=2.0):
         self.optimizers = list(optimizers)
@@ -139,6 +140,8 @@ class FusedClipSGD:
         if not idx:
             return None
         hip.require_gpu(self.params[idx[0]].grad)
+        if torch.cuda.is_current_stream_capturing():   # (a first step's momentum buffers would come out of the graph's pool, and their zeros with it)
+            raise hip.LgdHipError("the fused step's table (addresses, learning rates) is the host's of this call: it cannot be captured into a graph")
         self._buffers(idx)
         chunk = int(hip.load().lgd_sgd_chunk_elems())
         ii = np.asarray(idx, dtype=np.int64)

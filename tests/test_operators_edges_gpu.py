@@ -148,3 +148,27 @@ def test_the_step_refuses_tensors_that_no_longer_fit(limit):
         with pytest.raises(hip.LgdHipError, match="fused SGD needs"):
             fused.step()
         assert all(torch.equal(p, b) for p, b in zip(ps, before)), what
+
+
+@pytest.mark.parametrize("clip", [dict(), dict(clip_value=0.5), dict(clip_norm=0.5)])
+@pytest.mark.parametrize("count", [6, 90])
+def test_a_step_is_not_captured(count, clip):
+    """with any kind of clipping: the table is the host's of the call; a first step neither, which would leave its buffers in the graph's memory; afterwards
+    the step goes on eagerly"""
+    from lgd_amd import hip, optim
+    ps, opts = _sgd(count)
+    fused = optim.FusedClipSGD(opts, **clip)
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    for first in (True, False):
+        before = [p.detach().clone() for p in ps]
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(hip.LgdHipError, match="captured"):
+            with torch.cuda.graph(graph):
+                fused.step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, b) for p, b in zip(ps, before))
+        assert not first or not any(o.state for o in opts)
+        fused.step()
+        assert not any(torch.equal(p, b) for p, b in zip(ps, before))
