@@ -64,6 +64,10 @@ int type_code(const Tensor& t) {   // LGD_F32 / LGD_BF16 / LGD_F16, -1: none of 
     }
 }
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+// a tangent of forward-mode differentiation: these operators would drop it, which is a derivative of zero
+void refuse_dual(const Tensor& t, const char* what) {
+    if (t.defined() && t._fw_grad(0).defined()) refuse(what, " has no forward-mode derivative: an input carries a tangent");
+}
 Tensor dense(const Tensor& t) { return t.is_contiguous(at::MemoryFormat::ChannelsLast) ? t : t.contiguous(at::MemoryFormat::ChannelsLast); }
 void* ptr_or_null(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
@@ -98,7 +102,9 @@ void gn_check(const variable_list& xs, int64_t groups, const Tensor& w, const Te
             refuse("maps of one call are strided, of one type and on one device, got ", x.layout(), " ", x.scalar_type(), " ", x.device(), " beside ",
                    x0.scalar_type(), " ", x0.device());
         for (int d = 0; d < 4; ++d) if (x.size(d) > INT32_MAX) refuse("a map's sizes are below 2^31, got ", x.sizes());
+        refuse_dual(x, "group_norm_act");
     }
+    refuse_dual(w, "group_norm_act"); refuse_dual(b, "group_norm_act");
     const int64_t C = x0.size(1);
     if (groups < 1 || C < 1 || groups > C || C % groups) refuse(C, " channels do not split into ", groups, " groups");
     for (const Tensor* p : {&w, &b})
@@ -177,6 +183,8 @@ struct GnBackward : public Node {
         bool any = false;
         for (const Tensor& d : dys) any = any || d.defined();
         if (!any) return out;
+        for (const Tensor& d : dys)
+            if (d.defined() && d._fw_grad(0).defined()) throw std::runtime_error("group_norm_act has no forward-mode derivative: an output's gradient carries a tangent");
         refuse_capture();
         {
             at::AutoDispatchBelowADInplaceOrView below;
@@ -321,6 +329,7 @@ Tensor norm_of(const std::vector<Tensor>& ts, int norm_type, bool clip, double m
         if (t.layout() != at::kStrided || type < 0 || t.device() != dev)
             refuse("gradient norms take strided fp32, bf16 or fp16 tensors on one device, got ",
                    t.layout(), " ", t.scalar_type(), " ", t.device(), " (the first is on ", dev, ")");
+        refuse_dual(t, "the norm of gradients");
         flat.push_back(t.is_non_overlapping_and_dense() ? t : t.contiguous());   // any dense order is one run of memory
         rec.push_back({flat.back().data_ptr(), t.numel(), type, 0});
     }

@@ -348,7 +348,8 @@ def group_norm_act(xs, groups, weight=None, bias=None, act="relu", eps=1e-5):
     """act(nn.GroupNorm(groups, C, eps)(x)) of a list of CHANNELS-LAST maps (B,C,H_l,W_l), fp32 / bf16 / fp16, with ONE module over all of
     them (group_norm_relu is the NCHW fp32 form): act "none", "relu" or "silu"; weight / bias (C,) fp32, bf16 or fp16, or None.  Maps that are
     not dense in torch.channels_last order are copied into it; the outputs and the input gradients are channels-last, in the maps' type,
-    rounded once (statistics and the sign under a ReLU are 64-bit).  A map without elements gives one without elements.  First derivatives only.
+    rounded once (statistics and the sign under a ReLU are 64-bit).  A map without elements gives one without elements.  First derivatives
+    only: differentiating again, or in forward mode, raises.
     A backward captured into a graph takes leaves that no older graph from another stream holds (refused otherwise).
     The checks, the allocations and the autograd node are csrc/host.cpp: on small maps they are most of what a call costs."""
     code = _GN_ACTS.get(act)

@@ -68,6 +68,17 @@ def test_a_derivative_by_the_output_gradient_raises(form):
         torch.autograd.grad(g.square().sum(), [dy])
 
 
+def test_a_tangent_of_the_output_gradient_raises():
+    """forward over reverse: an error, not an input gradient without a tangent"""
+    import torch.autograd.forward_ad as fw
+    from lgd_amd import ops
+    x, dy = _map("nchw"), _rand((2, 8, 5, 6), 5)
+    y, = ops.group_norm_act([x], 2)
+    with fw.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(y, [x], fw.make_dual(dy, torch.ones_like(dy)))
+
+
 def _sgd(count, seed=7):
     g = torch.Generator().manual_seed(seed)
     ps = [torch.nn.Parameter(torch.randn(5 + 3 * i, generator=g).to(DEV)) for i in range(count)]
