@@ -140,11 +140,18 @@ variable_list gn_forward(const variable_list& xs, int groups, int act, double ep
     return ys;
 }
 
-// gradients computed under create_graph depend on x in a way no graph holds: differentiating them again must raise
-struct GnNoSecond : public Node {
-    variable_list apply(variable_list&&) override { throw std::runtime_error("group_norm_act has no second derivative"); }
-    std::string name() const override { return "GroupNormActNoSecondDerivative"; }
+// stands behind a result that depends on its inputs in a way no graph holds: differentiating it must raise
+struct NoDerivative : public Node {
+    std::string who, what;
+    NoDerivative(std::string w, std::string t) : who(std::move(w)), what(std::move(t)) {}
+    variable_list apply(variable_list&&) override { throw std::runtime_error(who + " has no " + what); }
+    std::string name() const override { return "NoDerivative"; }
 };
+std::shared_ptr<Node> no_derivative(const char* who, const char* what, torch::autograd::edge_list&& edges) {
+    std::shared_ptr<Node> node(new NoDerivative(who, what), torch::autograd::deleteNode);
+    node->set_next_edges(std::move(edges));
+    return node;
+}
 
 struct GnBackward : public Node {
     std::vector<SavedVariable> x;
@@ -196,8 +203,7 @@ struct GnBackward : public Node {
             for (const Tensor& t : dys)
                 if (t.defined() && t.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(t));
             if (!edges.empty()) {
-                auto node = std::shared_ptr<GnNoSecond>(new GnNoSecond(), torch::autograd::deleteNode);
-                node->set_next_edges(std::move(edges));
+                const auto node = no_derivative("group_norm_act", "second derivative", std::move(edges));   // (of gradients computed under create_graph)
                 for (Tensor& t : out) if (t.defined()) torch::autograd::set_history(t, node);
             }
         }
@@ -514,8 +520,14 @@ PyObject* py_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     try {
         const std::vector<Tensor> ts = tensors_of(seq.o, grads == 1);
         if (ts.empty()) Py_RETURN_NONE;
-        const Tensor out = norm_of(ts, (int)code, clip, max_norm);
+        Tensor out = norm_of(ts, (int)code, clip, max_norm);
         if (!out.defined()) Py_RETURN_FALSE;
+        if (!clip && at::GradMode::is_enabled()) {
+            torch::autograd::edge_list edges;
+            for (const Tensor& t : ts)
+                if (t.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(t));
+            if (!edges.empty()) torch::autograd::set_history(out, no_derivative("grad_norm", "derivative", std::move(edges)));
+        }
         return THPVariable_Wrap(out);
     } catch (const Refused& e) {
         PyErr_SetString(api.error, e.what());

@@ -35,7 +35,8 @@ def _norm_code(norm_type):
 
 def grad_norm(tensors, norm_type=2.0):
     """norm over every element of every tensor (fp32 / bf16 / fp16, mixed) as ONE vector -> 0-dim fp32 tensor on their device, no host sync:
-    norm_type 2, 1 or inf.  Sums are 64-bit and run in a fixed order.  A NaN anywhere gives NaN.  No tensors: 0 on the CPU."""
+    norm_type 2, 1 or inf.  Sums are 64-bit and run in a fixed order.  A NaN anywhere gives NaN.  No tensors: 0 on the CPU.
+    It has no derivative: differentiating the norm of tensors that are part of a graph raises."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     return _norm(hip.host().norm(tensors, False, _norm_code(norm_type), None), tensors)
 

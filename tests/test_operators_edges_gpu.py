@@ -68,6 +68,22 @@ def test_a_derivative_by_the_output_gradient_raises(form):
         torch.autograd.grad(g.square().sum(), [dy])
 
 
+def test_a_derivative_of_the_norm_raises():
+    """a gradient penalty by grad_norm: an error, not a penalty that is left out; without a graph the norm has none either"""
+    from lgd_amd import optim
+    w = _rand((8, 8), 6).requires_grad_(True)
+    g, = torch.autograd.grad((w * w * w).sum(), [w], create_graph=True)
+    n = optim.grad_norm([g, torch.ones(3, device=DEV)])
+    assert n.requires_grad
+    with pytest.raises(RuntimeError, match="no derivative"):
+        ((w * w).sum() + n).backward()
+    with torch.no_grad():
+        assert torch.equal(optim.grad_norm([g, torch.ones(3, device=DEV)]), n) and not optim.grad_norm([g]).requires_grad
+    assert not optim.grad_norm([g.detach()]).requires_grad
+    w.grad = g
+    assert not optim.clip_grad_norm_([w], 1.0).requires_grad
+
+
 def test_a_tangent_of_the_output_gradient_raises():
     """forward over reverse: an error, not an input gradient without a tangent"""
     import torch.autograd.forward_ad as fw
