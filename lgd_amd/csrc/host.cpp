@@ -17,6 +17,7 @@
 #include <torch/csrc/autograd/saved_variable.h>
 
 #include <algorithm>
+#include <mutex>
 #include <sstream>
 #include <vector>
 
@@ -153,6 +154,7 @@ std::shared_ptr<Node> no_derivative(const char* who, const char* what, torch::au
     return node;
 }
 
+// What is saved is read and released under the node's lock: two threads may differentiate one graph, one of them releasing it
 struct GnBackward : public Node {
     std::vector<SavedVariable> x;
     SavedVariable w, b;
@@ -162,9 +164,11 @@ struct GnBackward : public Node {
 
     std::string name() const override { return "GroupNormActBackward"; }
     void release_variables() override {
-        for (auto& v : x) v.reset_data();
-        w.reset_data(); b.reset_data();
-        stats.reset();
+        std::vector<SavedVariable> xs;   // let go of behind the lock: the last reference of a tensor may call into Python
+        SavedVariable wv, bv;
+        Tensor st;
+        const std::lock_guard<std::mutex> lock(mutex_);
+        std::swap(xs, x); std::swap(wv, w); std::swap(bv, b); std::swap(st, stats);
         released = true;
     }
     // A leaf whose gradient accumulator belongs to an older graph, made on another stream, would have the engine make that stream wait inside the capture:
@@ -181,11 +185,15 @@ struct GnBackward : public Node {
         }
     }
     variable_list apply(variable_list&& dys) override {
-        TORCH_CHECK(!released, "group_norm_act: the graph has been freed; backward a second time needs retain_graph=True the first time");
         const bool again = at::GradMode::is_enabled();   // create_graph
         variable_list xs;
-        for (auto& v : x) xs.push_back(v.unpack());
-        const Tensor wv = w.unpack(), bv = b.unpack();
+        Tensor wv, bv, st;
+        {
+            const std::lock_guard<std::mutex> lock(mutex_);
+            TORCH_CHECK(!released, "group_norm_act: the graph has been freed; backward a second time needs retain_graph=True the first time");
+            for (auto& v : x) xs.push_back(v.unpack());
+            wv = w.unpack(); bv = b.unpack(); st = stats;
+        }
         variable_list out(xs.size() + 2);
         bool any = false;
         for (const Tensor& d : dys) any = any || d.defined();
@@ -195,7 +203,7 @@ struct GnBackward : public Node {
         refuse_capture();
         {
             at::AutoDispatchBelowADInplaceOrView below;
-            run(xs, wv, bv, dys, out);
+            run(xs, wv, bv, st, dys, out);
         }
         if (again) {
             torch::autograd::edge_list edges;
@@ -209,7 +217,7 @@ struct GnBackward : public Node {
         }
         return out;
     }
-    void run(const variable_list& saved, const Tensor& w0, const Tensor& b0, const variable_list& dys, variable_list& out) {
+    void run(const variable_list& saved, const Tensor& w0, const Tensor& b0, const Tensor& st, const variable_list& dys, variable_list& out) {
         const size_t nx = saved.size();
         variable_list xs;   // (hooks on saved tensors may hand them back in another order)
         for (const Tensor& x : saved) xs.push_back(dense(x));
@@ -239,7 +247,7 @@ struct GnBackward : public Node {
             Tensor ws;
             if (n) ws = at::empty({(int64_t)n}, xs[0].options().dtype(at::kByte).memory_format(at::MemoryFormat::Contiguous));
             check(api.gn_bwd(c.x.data(), dy.data(), c.hw.data(), c.L, c.B, c.C, groups, c.type, ptr_or_null(wv), ptr_or_null(bv), c.ptype, act,
-                             stats.data_ptr<double>(), ptr_or_null(ws), want_x ? dx.data() : nullptr, ptr_or_null(dw), ptr_or_null(db), stream_of(xs[0])),
+                             st.data_ptr<double>(), ptr_or_null(ws), want_x ? dx.data() : nullptr, ptr_or_null(dw), ptr_or_null(db), stream_of(xs[0])),
                   "lgd_gn_act_bwd");
         }
         for (size_t i = 0; i < nx; ++i) if (task_should_compute_output(i)) out[i] = dxs[i];

@@ -68,6 +68,34 @@ def test_a_derivative_by_the_output_gradient_raises(form):
         torch.autograd.grad(g.square().sum(), [dy])
 
 
+def test_threads_that_differentiate_one_graph():
+    """two threads run backward over one graph, a third one releases it in between: the right gradients or the error of a freed graph, nothing else"""
+    import threading
+    from lgd_amd import ops
+    x, (w, b), dy = _map("nchw"), _parameters("trainable"), _rand((2, 8, 5, 6), 5)
+    want = torch.autograd.grad(ops.group_norm_act([x], 2, w, b, act="silu")[0], [x, w, b], dy)
+    torch.cuda.synchronize()
+    for keep in (True, False):
+        y, = ops.group_norm_act([x], 2, w, b, act="silu")
+        got, errors, start = [], [], threading.Barrier(3)
+
+        def work(times, retain):
+            start.wait()
+            for _ in range(times):
+                try:
+                    got.append(torch.autograd.grad(y, [x, w, b], dy, retain_graph=retain))
+                except RuntimeError as e:
+                    errors.append(str(e))
+        threads = [threading.Thread(target=work, args=a) for a in ((20, True), (20, True), (1, keep))]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        assert len(got) + len(errors) == 41 and all("freed" in e for e in errors) and (not keep or not errors) and got
+        assert all(torch.equal(g, v) for grads in got for g, v in zip(grads, want))
+
+
 def test_a_derivative_of_the_norm_raises():
     """a gradient penalty by grad_norm: an error, not a penalty that is left out; without a graph the norm has none either"""
     from lgd_amd import optim
