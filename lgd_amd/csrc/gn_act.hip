@@ -11,8 +11,10 @@
 // unaligned: the vector type below carries the element's alignment and gfx950 runs global memory in unaligned access mode.
 //
 // Precision.  Sums of x and x^2 are fp64 (gfx950 runs fp64 FMA at the rate of unpacked fp32), the statistics stay fp64, and z = x (r gamma) +
-// (beta - mu r gamma) is ONE fp64 FMA per element: the sign a ReLU's gradient hangs on is decided in 64 bits.  Sums of the backward are fp32 over one
-// thread's rows of a chunk (<= a few hundred terms), fp64 across its workgroup, one fp32 word per chunk, fp64 across those.  Outputs are rounded once (fp32 -> 16 bits).
+// (beta - mu r gamma) is ONE fp64 FMA per element: the sign a ReLU's gradient hangs on is decided in 64 bits.  Sums of the backward begin in fp32: at
+// most kGaTerms rows of a thread, which then join a 64-bit sum (a thread has 160 rows at 340 MB, tens of thousands at the largest sizes); from there on
+// they are fp64 but for the words that pass between threads, workgroups and kernels, each one rounding to fp32.  Outputs are rounded once
+// (fp32 -> 16 bits).
 #include "gn_act.h"
 
 #include <type_traits>
@@ -23,6 +25,7 @@ namespace lgd {
 // what they move), 768 197 / 345 (three on some CUs, four on others), 1024 177 / 299
 constexpr int kGaWorkgroups = 512;
 constexpr int kGaU = 4, kGaUB = 2;     // vectors (of x; of x and dy each) of a thread in flight
+constexpr int kGaTerms = 256;          // terms that the backward adds in fp32 before they join a 64-bit sum
 constexpr int kGaRecordsU = 8;         // records of a thread in flight
 constexpr int kGaThreads = 256;        // of the kernels in between
 constexpr int kGaMax = 320;            // of the streaming kernels: 192, 256 or 320, whichever has a vector for most of its threads
@@ -115,7 +118,7 @@ __device__ __forceinline__ GaThread ga_thread(const GaArgs& a, int E) {
 
 // A thread's way through its vectors, U in flight: begin() issues the first block's loads (kernels that have something to compute first call it in
 // front of that), run() consumes them and goes on.  load(e): a whole vector's registers; use(regs, e, count); part(e, count): the one vector that the
-// sample's end cuts, zero filled, comes last
+// sample's end cuts, zero filled, comes last; turn(): behind every U vectors
 template <int V, int U, typename Regs> struct GaWalk {
     int s, K, block, step, send;
     unsigned e;   // element offset of super-row s (wraps only behind the last one, where it is not used)
@@ -130,17 +133,22 @@ template <int V, int U, typename Regs> struct GaWalk {
         e = (unsigned)s * a.P + t.v * V;
         loads(a, load);
     }
-    template <typename Load, typename Part, typename Use>
-    __device__ __forceinline__ void run(const GaArgs& a, const GaWhere& q, const GaThread& t, int E, Load load, Part part, Use use) {
+    template <typename Load, typename Part, typename Use, typename Turn>
+    __device__ __forceinline__ void run(const GaArgs& a, const GaWhere& q, const GaThread& t, int E, Load load, Part part, Use use, Turn turn) {
         while (s < send) {
             #pragma unroll
             for (int u = 0; u < U; ++u) if (s + u * a.R < send) use(v[u], e + u * step, V);
             s += K * block; e += (unsigned)(K * U) * step;
             loads(a, load);
+            turn();
         }
         if (a.P == a.C || !t.on) return;   // samples are whole vectors
         const unsigned cut = (unsigned)send * a.P + t.v * V;
         if (cut < (unsigned)E && send / block % K == q.k && send % a.R == t.r) use(part(cut, E - cut), cut, E - cut);
+    }
+    template <typename Load, typename Part, typename Use>
+    __device__ __forceinline__ void run(const GaArgs& a, const GaWhere& q, const GaThread& t, int E, Load load, Part part, Use use) {
+        run(a, q, t, E, load, part, use, [] {});
     }
 };
 
@@ -414,7 +422,11 @@ template <int V, int S> struct GaCoef {
 template <typename T, int ACT, int S>
 __global__ __launch_bounds__(kGaMax) void ga_bwd_stats_kernel(GaArgs a) {
     constexpr int V = Vec16<T>::V, W = V / S;
-    __shared__ float2 sh[V * kGaPad], shg[S * kGaPad];
+    // 64-bit sums of the blocks of kGaTerms terms before the last (written by long chunks only: in registers they cost 16-bit types a wave per SIMD, 12 - 17 %
+    // on odd channels); then the threads' sums and, with gamma, the groups' pieces
+    __shared__ double2 acc[V * kGaPad];
+    float2* sh = reinterpret_cast<float2*>(acc);
+    float2* shg = sh + V * kGaPad;
     const GaWhere q = ga_locate(a, blockIdx.x);
     const int E = a.E[q.l];
     const GaThread t = ga_thread<V>(a, E);
@@ -428,6 +440,7 @@ __global__ __launch_bounds__(kGaMax) void ga_bwd_stats_kernel(GaArgs a) {
     float s0[V], s1[V];
     #pragma unroll
     for (int i = 0; i < V; ++i) s0[i] = s1[i] = 0.f;
+    int turns = 0, blocks = 0;
     walk.run(a, q, t, E, load,
         [&](unsigned e, int n) { return GaXD<T>{ga_load_part(px + e, n), ga_load_part(pd + e, n)}; },
         [&](const GaXD<T>& v, unsigned, int) {
@@ -438,7 +451,30 @@ __global__ __launch_bounds__(kGaMax) void ga_bwd_stats_kernel(GaArgs a) {
                 const float xh = ga_xhat(x[i], k.at(i)), g = ga_grad<ACT>(d[i], x[i], xh, k.at(i), k.ga[i], k.be[i]);
                 s0[i] += g; s1[i] = __builtin_fmaf(g, xh, s1[i]);
             }
+        },
+        [&] {
+            if (++turns < kGaTerms / kGaUB) return;
+            turns = 0;
+            #pragma unroll
+            for (int i = 0; i < V; ++i) {
+                double2& t = acc[i * kGaPad + threadIdx.x];
+                const double2 before = blocks ? t : make_double2(0.0, 0.0);
+                t = make_double2(before.x + (double)s0[i], before.y + (double)s1[i]);
+                s0[i] = s1[i] = 0.f;
+            }
+            ++blocks;
         });
+    // (the same for the whole workgroup: no thread of a shorter chunk has got that far)
+    if (E / a.P + 1 > (kGaTerms - kGaUB) * a.R * a.K[q.l]) {
+        if (blocks) {
+            #pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const double2 t = acc[i * kGaPad + threadIdx.x];
+                s0[i] = (float)(t.x + (double)s0[i]); s1[i] = (float)(t.y + (double)s1[i]);
+            }
+        }
+        __syncthreads();
+    }
     #pragma unroll
     for (int i = 0; i < V; ++i) sh[i * kGaPad + threadIdx.x] = make_float2(s0[i], s1[i]);
     if (a.fused) {   // with gamma, for the groups

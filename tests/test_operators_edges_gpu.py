@@ -1,4 +1,5 @@
-"""Calls of the channels-last GroupNorm, the gradient norms and the fused SGD step at their edges: differentiating again, optimizer states that come and go."""
+"""Calls of the channels-last GroupNorm, the gradient norms and the fused SGD step at their edges: differentiating again, optimizer states that come and go,
+long sums."""
 import copy
 
 import pytest
@@ -227,3 +228,36 @@ def test_a_step_is_not_captured(count, clip):
         assert not first or not any(o.state for o in opts)
         fused.step()
         assert not any(torch.equal(p, b) for p, b in zip(ps, before))
+
+
+def test_parameter_gradients_over_millions_of_pixels():
+    """dgamma and dbeta of like-signed terms, 2^22 pixels: x = 1 and -1 in turn (mean 0, variance 1), dy = c in the even channels and c x in the odd ones, so that
+    dbeta = n c or 0, dgamma = 0 or n c r with r = 1 / sqrt(1 + eps).  At most 256 terms are added in fp32: 256 U, and a few U for the terms and the
+    sums' roundings"""
+    from lgd_amd import ops
+    n, C, c = 2048 * 2048, 256, torch.tensor(0.6, dtype=torch.float32)
+    x = torch.ones(1, 2048, 2048, C, device=DEV)
+    x[:, :, 1::2] = -1.0
+    dy = torch.full((1, 2048, 2048, C), float(c), device=DEV)
+    dy[..., 1::2] *= x[..., 1::2]
+    x, dy = x.permute(0, 3, 1, 2), dy.permute(0, 3, 1, 2)
+    w, b = torch.ones(C, device=DEV, requires_grad=True), torch.zeros(C, device=DEV, requires_grad=True)
+    y, = ops.group_norm_act([x], 32, w, b, act="none", eps=1e-5)
+    dw, db = torch.autograd.grad(y, [w, b], dy)
+    total, r = n * float(c), (1 + 1e-5) ** -0.5
+    assert float((db[0::2].double() - total).abs().max()) <= 264 * U * total
+    assert float((dw[1::2].double() - total * r).abs().max()) <= 264 * U * total
+    assert float(db[1::2].abs().max()) <= 264 * U * total and float(dw[0::2].abs().max()) <= 264 * U * total
+
+
+@pytest.mark.parametrize("C,G,dtype,act", [(33, 3, torch.bfloat16, "silu"), (24, 2, torch.float16, "relu"), (20, 5, torch.float32, "none")])
+def test_group_norm_act_over_long_chunks(C, G, dtype, act):
+    """maps of 0.7 GB, where a thread's sums are cut into blocks of 256 terms: odd rows over several vectors, one and several groups a vector; all results against
+    64 bits, at the tolerances of the small maps (256 U of the terms' magnitudes)"""
+    from test_operators_gpu import _check, _params, _run
+    side = int((0.7e9 / C / dtype.itemsize) ** 0.5)
+    g = torch.Generator(device=DEV).manual_seed(C)
+    x, dy = ((torch.randn(1, side, side + 3, C, device=DEV, generator=g) * k + m).to(dtype).permute(0, 3, 1, 2) for k, m in ((1.3, 0.4), (1.0, 0.2)))
+    w, b = _params(C, torch.float32, 9)
+    ys, dxs, dw, db = _run([x], G, w, b, act, 1e-5, [dy])
+    _check([x], G, w, b, act, 1e-5, [dy], ys, dxs, dw, db)
