@@ -675,8 +675,11 @@ static int ga_plan(GaArgs& a, const int32_t* hw, int L, int B, int C, int G, int
         a.E[l] = (int)e; a.HW[l] = (int)n;
         total += e * B * size;
     }
-    const long long bytes = total / kGaWorkgroups < 16384 ? 16384 : total / kGaWorkgroups;
-    const long long block = 16LL * kGaU * a.R * a.cols;   // (U vectors a thread)
+    // a chunk is `bytes` of a sample for each of its nCB workgroups, and a block of U super-rows a thread at least: more chunks than that hold nothing, and
+    // leave records of zeros (2 x 2047 x 30 x 30 fp32, 7 column blocks: forward 45 -> 20 us, both directions 178 -> 53; 4 x 2048 x 40 x 40, 2 blocks of
+    // whole groups: 84 -> 79)
+    const long long bytes = (total / kGaWorkgroups < 16384 ? 16384 : total / kGaWorkgroups) * a.nCB;
+    const long long block = (long long)kGaU * a.R * a.P * size;
     const int rec = a.mixed ? a.nCB : 1;
     const long long cap = kGaFusedRecords / ((long long)G * rec);
     long long w = 0, wf = 0;
@@ -688,7 +691,7 @@ static int ga_plan(GaArgs& a, const int32_t* hw, int L, int B, int C, int G, int
         wf += B * (k < cap ? k : cap);
     }
     // one kernel less where the records are few enough without leaving the chip short of workgroups
-    a.fused = G <= kGaFusedG && cap >= 1 && (wf == w || wf >= 384);
+    a.fused = G <= kGaFusedG && cap >= 1 && (wf == w || wf * a.nCB >= 384);
     if ((w + C / kGaParamC + 1) * a.NT > 0xffffffffLL || w * a.nCB > 0x3fffffffLL || (!a.fused && (long long)L * B * G * kGaThreads > 0xffffffffLL) ||
         (long long)L * B * G > 0x3fffffffLL)
         return LGD_EINVAL;   // (threads of a launch; 32-bit numbers of records and statistics)

@@ -6,6 +6,14 @@ import torch.autograd.forward_ad as fw
 from lgd_amd import hip, ops, optim
 
 
+@pytest.fixture(scope="module", autouse=True)
+def built():
+    import os
+    if not os.path.exists(hip.lib_path()):
+        import __graft_entry__ as g
+        g.build()
+
+
 @pytest.mark.parametrize("which", ["map", "second map", "weight", "bias", "gradient", "clipped gradient"])
 def test_forward_mode_is_refused(which):
     """an input with a tangent: an error, not an output without one"""
@@ -21,3 +29,17 @@ def test_forward_mode_is_refused(which):
                 optim.clip_grad_norm_([p], 1.0)
             else:
                 ops.group_norm_act([dual(x, "map"), dual(y, "second map")], 2, dual(w, "weight"), dual(b, "bias"))
+
+
+# batch, channels, groups, map, type, bytes of an element: rows of more than 320 vectors, that a vector of 16 bytes divides or not
+WIDE = [(8, 2049, 3, (16, 16), 1, 2), (8, 1025, 5, (32, 32), 1, 2), (2, 2047, 23, (30, 30), 0, 4), (8, 1331, 11, (16, 16), 2, 2), (3, 517, 11, (60, 60), 1, 2),
+        (4, 2048, 32, (40, 40), 0, 4), (2, 4096, 32, (40, 40), 1, 2), (1, 5001, 3, (64, 64), 0, 4)]
+
+
+@pytest.mark.parametrize("B,C,G,hw,dtype,size", WIDE, ids=str)
+def test_workspace_of_wide_rows_stays_below_the_maps(B, C, G, hw, dtype, size):
+    """a row over several column blocks: what the workgroups leave for one another is less than the maps themselves"""
+    shape = hip.int_array(list(hw))
+    maps = B * C * hw[0] * hw[1] * size
+    for backward in (0, 1):
+        assert hip.load().lgd_gn_act_ws_bytes(shape, 1, B, C, G, dtype, backward) < maps
