@@ -26,16 +26,25 @@ constexpr int kSgdChunk = 4096;  // elements per workgroup: 256 threads x 4 floa
 // the accesses stay dwordx4 (the compiler emits them for this type); round 2 sent such tensors down the scalar path.
 typedef float sgd_f4u __attribute__((ext_vector_type(4), aligned(4)));
 
-// global accesses (the pointers come out of a table: generic to the compiler otherwise), streaming: nothing of a step's six
-// transfers is used again in it (37 M parameters, clipped by norm: 167 us a step, 198 - 205 with plain loads, plain stores or both)
+// Global accesses (the pointers come out of a table: generic to the compiler otherwise).  Loads stream past the caches; stores do (ST) where the gradients have
+// just been read for their norm, and are plain in the step by value.  37 M parameters, us:
+//   by norm, alone: 167; 198 - 205 with plain loads, plain stores or both
+//   by value, behind a backward in training: 179; 190 with plain loads, 187 with plain loads and streaming stores, 213 with both streaming
 typedef __attribute__((address_space(1))) const sgd_f4u* sgd_gptr;
 typedef __attribute__((address_space(1))) sgd_f4u* sgd_gptr_rw;
 typedef __attribute__((address_space(1))) const lgd_vf4* sgd_gptr4;
 typedef __attribute__((address_space(1))) lgd_vf4* sgd_gptr4_rw;
 __device__ __forceinline__ float4 sgd_load4(const float* p) { const lgd_vf4 v = __builtin_nontemporal_load((sgd_gptr4)p); return make_float4(v.x, v.y, v.z, v.w); }
 __device__ __forceinline__ sgd_f4u sgd_loadu(const float* p) { return __builtin_nontemporal_load((sgd_gptr)p); }
-__device__ __forceinline__ void sgd_store4(float* p, const float4& f) { const lgd_vf4 v = {f.x, f.y, f.z, f.w}; __builtin_nontemporal_store(v, (sgd_gptr4_rw)p); }
-__device__ __forceinline__ void sgd_storeu(float* p, const sgd_f4u& v) { __builtin_nontemporal_store(v, (sgd_gptr_rw)p); }
+template <bool ST> __device__ __forceinline__ void sgd_store4(float* p, const float4& f) {
+    const lgd_vf4 v = {f.x, f.y, f.z, f.w};
+    if constexpr (ST) __builtin_nontemporal_store(v, (sgd_gptr4_rw)p);
+    else *(sgd_gptr4_rw)p = v;
+}
+template <bool ST> __device__ __forceinline__ void sgd_storeu(float* p, const sgd_f4u& v) {
+    if constexpr (ST) __builtin_nontemporal_store(v, (sgd_gptr_rw)p);
+    else *(sgd_gptr_rw)p = v;
+}
 
 // by value: the clamped gradient, NaN stays NaN (as torch.clamp); by norm: `clip` is the optimizer's factor
 template <bool NORM> __device__ __forceinline__ float sgd_clipped(float g, float clip) {
@@ -75,10 +84,10 @@ __device__ __forceinline__ void sgd_chunk(const lgd_sgd_tensor& t, long long bas
                 const float b = mu * mm[j] + d;
                 gg[j] = c; mm[j] = b; pp[j] = __builtin_fmaf(-lr, b, pp[j]);
             }
-            sgd_store4(t.p + i, p[k]);
+            sgd_store4<NORM>(t.p + i, p[k]);
             sgd_f4u go; go.x = g[k].x; go.y = g[k].y; go.z = g[k].z; go.w = g[k].w;
-            if (write_g) sgd_storeu(t.g + i, go);
-            sgd_store4(t.m + i, m[k]);
+            if (write_g) sgd_storeu<NORM>(t.g + i, go);
+            sgd_store4<NORM>(t.m + i, m[k]);
         }
     } else {
         clip = clip_of();
