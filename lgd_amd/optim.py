@@ -19,6 +19,7 @@ _TENSOR_DT = np.dtype([("p", "<u8"), ("g", "<u8"), ("m", "<u8"), ("n", "<i8"), (
                        ("reserved", "<i4")])  # mirror of lgd_sgd_tensor (include/lgd_hip.h), 48 bytes
 assert _TENSOR_DT.itemsize == 48
 
+MAX_GROUPS = 16   # LGD_MAX_SGD_GROUPS
 _NORMS = {2.0: 0, 1.0: 1, float("inf"): 2}   # LGD_NORM_*
 
 
@@ -65,12 +66,14 @@ def _norm(got, tensors):
 
 def supported(optimizers, clip):
     """the fused step covers what the reference's configs use: SGD (dampening 0, no Nesterov, not maximize) on fp32 CUDA parameters,
-    gradient clipping off, CLIP_TYPE 'value', or 'full_model' (by the norm of each optimizer's whole gradient; NORM_TYPE 1, 2 or inf); anything
-    else stays on torch's own multi-tensor path."""
+    gradient clipping off, CLIP_TYPE 'value', or 'full_model' (by the norm of each optimizer's whole gradient; NORM_TYPE 1, 2 or inf; at most 16
+    optimizers that share no parameter); anything else stays on torch's own multi-tensor path."""
     if clip.ENABLED and clip.CLIP_TYPE not in ("value", "full_model"):
         return False
-    if clip.ENABLED and clip.CLIP_TYPE == "full_model" and not has_norm(clip.NORM_TYPE):
-        return False
+    if clip.ENABLED and clip.CLIP_TYPE == "full_model":
+        ids = [id(p) for o in optimizers for g in o.param_groups for p in g["params"]]
+        if not has_norm(clip.NORM_TYPE) or len(optimizers) > MAX_GROUPS or len(set(ids)) != len(ids):
+            return False
     for o in optimizers:
         if type(o) is not torch.optim.SGD:
             return False
@@ -105,7 +108,7 @@ class FusedClipSGD:
         n = len(self.params)
         if clip_norm is not None:
             _norm_code(norm_type)
-            if len({id(p) for p in self.params}) != n or not 1 <= len(self.optimizers) <= 16:
+            if len({id(p) for p in self.params}) != n or not 1 <= len(self.optimizers) <= MAX_GROUPS:
                 raise hip.LgdHipError("clipping by norm takes 1 to 16 optimizers (LGD_MAX_SGD_GROUPS) that share no parameter")
         self._numel = np.array([p.numel() for p in self.params], dtype=np.int64)
         self._m_ref = [None] * n   # momentum buffers

@@ -43,3 +43,20 @@ def test_workspace_of_wide_rows_stays_below_the_maps(B, C, G, hw, dtype, size):
     maps = B * C * hw[0] * hw[1] * size
     for backward in (0, 1):
         assert hip.load().lgd_gn_act_ws_bytes(shape, 1, B, C, G, dtype, backward) < maps
+
+
+def test_the_fused_step_by_norm_is_not_offered_for_what_it_refuses():
+    """a parameter in two optimizers, or more optimizers than it takes: the trainer stays on torch's step instead of failing"""
+    from types import SimpleNamespace
+    clip = lambda kind: SimpleNamespace(ENABLED=True, CLIP_TYPE=kind, CLIP_VALUE=1.0, NORM_TYPE=2.0)  # noqa: E731
+    param = lambda: SimpleNamespace(is_cuda=True, dtype=torch.float32, is_contiguous=lambda: True)  # noqa: E731
+    shared = param()
+
+    def sgd(*params):
+        o = torch.optim.SGD([torch.nn.Parameter(torch.zeros(1))], 0.1)
+        o.param_groups[0]["params"] = list(params)
+        return o
+    two, many = [sgd(shared, param()), sgd(param(), shared)], [sgd(param()) for _ in range(17)]
+    assert optim.supported(two, clip("value")) and optim.supported(many, clip("value"))
+    assert not optim.supported(two, clip("full_model")) and not optim.supported(many, clip("full_model"))
+    assert optim.supported(many[:16], clip("full_model"))
