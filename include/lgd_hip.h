@@ -656,8 +656,8 @@ int lgd_sgd_norm_step_host(const lgd_sgd_tensor* table_host, const int32_t* blk_
  *   stats: fp64 [L*B*G][2] (mean, 1/sqrt(var + eps)), 16-byte aligned, written by fwd, read by bwd;  ws: lgd_gn_act_ws_bytes(..., backward) bytes,
  *   16-byte aligned
  *   (0: none is needed, ws may be NULL; (size_t)-1: not a call these entries take).  It is a few percent of the maps, but where a row is over 5 KB and
- *   no multiple of 16 bytes: there every part of a row leaves sums of all channels (C^2 words a chunk: 0.2 - 0.9 of the maps at 16 x 16 to 60 x 60 pixels,
- *   more than them on a map of a few pixels)
+ *   no multiple of 16 bytes, or a group's part of it is over 5 KB: there every 5 KB of a row leave sums of all channels (C^2 words a chunk: 0.2 - 0.9 of
+ *   the maps for rows of 1000 - 2050 16-bit channels at 16 x 16 to 60 x 60 pixels, 4 times them for 8192 channels in 2 groups at 16 x 16, more on a few pixels)
  * backward: dx_host NULL: no input gradients; dgamma / dbeta NULL: not wanted.  Sums run in a fixed order (no atomics).
  */
 #define LGD_ACT_NONE 0

@@ -62,7 +62,7 @@ template <int ACT> __device__ __forceinline__ float ga_act(float z) {
     return z;
 }
 
-// The backward's constants of one channel (n = 1: of a lane; the mean and the inverse deviation belong to its group).  mean = hi + lo and
+// The backward's constants of a group: mean = hi + lo and
 // 1/deviation = r + rl are pairs of fp32 words: xh = (x - hi) r - lo r is as good as the fp64 form (x - hi is exact near the mean)
 struct GaGroup { float hi, lo, r, rl, nlr; };
 __device__ __forceinline__ GaGroup ga_group(double m, double r) {

@@ -21,8 +21,8 @@
 
 namespace lgd {
 
-// Workgroups of a streaming call, about: two for every CU, in step.  8 x 320 x 256 x 256 bf16, forward / backward us: 512 168 / 290 (5.1 TB/s of
-// what they move), 768 197 / 345 (three on some CUs, four on others), 1024 177 / 299
+// Workgroups of a streaming call, about: two for every CU, in step.  8 x 320 x 256 x 256 bf16, forward / backward us: 512 168 / 290 (6.0 and
+// 5.8 TB/s of the 3 and 5 times a map's bytes that they move), 768 197 / 345 (three on some CUs, four on others), 1024 177 / 299
 constexpr int kGaWorkgroups = 512;
 constexpr int kGaU = 4, kGaUB = 2;     // vectors (of x; of x and dy each) of a thread in flight
 constexpr int kGaTerms = 256;          // terms that the backward adds in fp32 before they join a 64-bit sum

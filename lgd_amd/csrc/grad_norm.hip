@@ -16,7 +16,10 @@ constexpr int kNormGrid = 1024;      // workgroups at most: 4 per CU
 constexpr int kNormUnroll = 4;       // 16-byte accesses of a thread in flight
 constexpr int kNormInline = 160;     // records in the kernel arguments (24 bytes each, under 4 KB)
 
-constexpr int kNormOnce = 8;         // chunks of a list that one workgroup takes alone: 3.7 us against 4.3 at 8 tensors of 1000, 5.4 against 4.3 at 16
+// Chunks of a list that one workgroup takes alone.  us, one workgroup / two launches, norm: tensors of 1000 2.5 / 4.1 at 2 chunks, 3.6 / 4.5 at 8, 4.4 / 4.4 at
+// 12, 5.3 / 4.5 at 16; whole chunks of 8192 fp32 2.9 / 4.4 at 2, 4.8 / 5.0 at 8, 5.0 / 4.8 at 9, 7.7 / 4.8 at 16 (clipping the same within 0.3): the two cross
+// at 8 - 12
+constexpr int kNormOnce = 8;
 
 struct NormEntry {
     void* p;

@@ -3,7 +3,7 @@
 // everything that runs on the GPU goes through the C ABI of include/lgd_hip.h, whose entry points lgd_amd/hip.py hands over (bind), so that both see
 // the same library.
 // What it is for: a training call on small maps costs the host two autograd.Function halves on two threads, 145 us on the MI355X host where the GPU needs
-// 25; a list of 160 gradients 62 us for 16; the step over 10 (160) tensors 37 (60) us in Python, 12 (26) here.
+// 25; a list of 160 gradients 62 us for 16; the step over 10 (160) tensors 37 (60) us in Python, 13 (26) here.
 #include <Python.h>
 
 #include <ATen/ATen.h>

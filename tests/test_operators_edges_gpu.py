@@ -261,3 +261,17 @@ def test_group_norm_act_over_long_chunks(C, G, dtype, act):
     w, b = _params(C, torch.float32, 9)
     ys, dxs, dw, db = _run([x], G, w, b, act, 1e-5, [dy])
     _check([x], G, w, b, act, 1e-5, [dy], ys, dxs, dw, db)
+
+
+@pytest.mark.parametrize("act", ["none", "silu"])
+@pytest.mark.parametrize("B,C,G,hws,dtype", [
+    (2, 2047, 23, [(30, 30)], torch.float32), (8, 1331, 11, [(16, 16)], torch.float16), (8, 2049, 3, [(16, 16), (1, 1)], torch.bfloat16),
+    (3, 517, 11, [(60, 60), (7, 9)], torch.bfloat16), (4, 2048, 32, [(40, 40)], torch.float32), (2, 4096, 32, [(40, 40), (3, 5)], torch.bfloat16),
+    (1, 4096, 1, [(25, 21)], torch.float32), (1, 1285, 257, [(200, 33)], torch.float32), (2, 5001, 3, [(2, 3)], torch.float32)], ids=str)
+def test_group_norm_act_wide_rows(B, C, G, hws, dtype, act):
+    """rows over two to sixteen column blocks, whole groups or cut ones: fewer chunks than workgroups, several maps; all results against 64 bits"""
+    from test_operators_gpu import _check, _maps, _params, _run
+    xs, dys = _maps(B, C, hws, dtype, 60, 1.3, 0.4), _maps(B, C, hws, dtype, 70)
+    w, b = _params(C, torch.float32, 80)
+    ys, dxs, dw, db = _run(xs, G, w, b, act, 1e-5, dys)
+    _check(xs, G, w, b, act, 1e-5, dys, ys, dxs, dw, db)
