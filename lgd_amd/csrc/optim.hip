@@ -23,7 +23,7 @@ constexpr int kSgdChunk = 4096;  // elements per workgroup: 256 threads x 4 floa
 // 4 floats at a 4-byte-aligned address: under DistributedDataParallel(gradient_as_bucket_view=True) a gradient is a view into a flat
 // bucket at the sum of the preceding parameters' sizes (train.py:279-281), i.e. dword- but not 16-byte-aligned as soon as one of them
 // has a size that is not a multiple of 4 (FCOS `scales`, the centerness bias).  gfx950 runs global memory in unaligned access mode, so
-// the accesses stay dwordx4 (the compiler emits them for this type); round 2 sent such tensors down the scalar path.
+// the accesses stay dwordx4 (the compiler emits them for this type).
 typedef float sgd_f4u __attribute__((ext_vector_type(4), aligned(4)));
 
 // Global accesses (the pointers come out of a table: generic to the compiler otherwise).  Loads stream past the caches; stores do (ST) where the gradients have
